@@ -318,6 +318,70 @@ int qssm_rmsnorm_bwd(const void* x, const float* w, const void* dy, const float*
                      int64_t rows, int64_t H, int64_t x_stride, int64_t dy_stride, int64_t dx_stride,
                      int dtype, void* stream);
 
+/*
+ * The 8-bit serving path and the residual norm around it.  No counterpart in the reference, whose layer computes
+ * RMSNorm, the projections and the residual's addition with torch operations (quick_ssm/layers.py:9-17, :76-107).
+ *
+ * Residual sum and RMS norm:
+ *     h[r, :] = x[r, :] + res[r, :]   (rounded to res_dtype, stored)
+ *     y[r, :] = h[r, :] * w / sqrt(mean(h[r, :]^2) + eps)
+ * x, y, dy, dx: `rows` rows of H elements of x_dtype; res, h, dh, dres: of res_dtype, which is x_dtype or QSSM_F32;
+ * w, dw: H elements of w_dtype.  Pitches in elements, any alignment, any H (16-byte aligned rows are fastest).
+ * Inputs may overlap each other but not the outputs, except that h may be res itself.
+ * forward : writes y, h and, if rstd != NULL, rstd[r] = 1/sqrt(mean(h^2)+eps).
+ * fp8     : writes h and, in place of y, its e4m3 values q (rows of q_stride bytes) with the scale of the 128 columns
+ *           from 128*b on at scales[r*scale_stride_row + b*scale_stride_blk].  res == NULL: h is x and is not written.
+ * backward: d = dh + rstd*(w*dy) - h*rstd^3*mean(h*w*dy) to dx (x_dtype) and dres (res_dtype), either of which may be
+ *           NULL; dw = sum_r dy*h*rstd in a fixed order (no atomics).  dh == NULL: zero.
+ *           ws: 16-byte aligned, at least qssm_add_rmsnorm_workspace_bytes(rows, H) bytes.
+ */
+size_t qssm_add_rmsnorm_workspace_bytes(int64_t rows, int64_t H);
+
+int qssm_add_rmsnorm_fwd(const void* x, const void* res, const void* w, void* y, void* h, float* rstd,
+                         int64_t rows, int64_t H, int64_t x_stride, int64_t res_stride, int64_t y_stride,
+                         int64_t h_stride, float eps, int x_dtype, int res_dtype, int w_dtype, void* stream);
+
+int qssm_add_rmsnorm_fp8(const void* x, const void* res, const void* w, void* q, float* scales, void* h,
+                         int64_t rows, int64_t H, int64_t x_stride, int64_t res_stride, int64_t q_stride,
+                         int64_t h_stride, int64_t scale_stride_row, int64_t scale_stride_blk, float eps,
+                         int x_dtype, int res_dtype, int w_dtype, void* stream);
+
+int qssm_add_rmsnorm_bwd(const void* h, const void* w, const void* dy, const void* dh, const float* rstd,
+                         void* dx, void* dres, void* dw, void* ws, size_t ws_bytes,
+                         int64_t rows, int64_t H, int64_t h_stride, int64_t dy_stride, int64_t dh_stride,
+                         int64_t dx_stride, int64_t dres_stride, int x_dtype, int res_dtype, int w_dtype,
+                         void* stream);
+
+/*
+ * Quantisation to e4m3 in blocks of QSSM_FP8_BLOCK = 128:
+ *     scale = max(amax, 2^-100) / 448     q = e4m3(v / scale), nearest even
+ * rows  : a scale for each 128 values of a row (activations; the scan's output before the output projection).
+ * blocks: a scale for each 128 x 128 block (weights), scales[bn*scale_stride_row + bk*scale_stride_blk].
+ * A block that holds an infinity or a NaN gets an infinite or NaN scale and gives NaN wherever it is used.
+ */
+#define QSSM_FP8_BLOCK 128
+
+int qssm_quant_fp8_rows(const void* x, void* q, float* scales, int64_t rows, int64_t K, int64_t x_stride,
+                        int64_t q_stride, int64_t scale_stride_row, int64_t scale_stride_blk, int dtype,
+                        void* stream);
+
+int qssm_quant_fp8_blocks(const void* w, void* q, float* scales, int64_t N, int64_t K, int64_t w_stride,
+                          int64_t q_stride, int64_t scale_stride_row, int64_t scale_stride_blk, int dtype,
+                          void* stream);
+
+/*
+ * Product of such operands:
+ *     y[m, n] = bias[n] + sum_b x_scales[m, b] * w_scales[n/128, b] * sum_{k in block b} x[m, k] * w[n, k]
+ * x [M, K], w [N, K]: e4m3, rows x_stride / w_stride bytes apart; both strides and both bases multiples of 16
+ * (QSSM_E_STRIDE otherwise).  Scales fp32 with strides of their own.  bias: N elements of bias_dtype, or NULL.
+ * y: out_dtype (any of the three), rows y_stride elements apart.  Sums in fp32, one rounding at the end.  K = 0 gives
+ * the bias.  status_word as above (an expired wait on a bulk copy).
+ */
+int qssm_matmul_fp8(const void* x, const float* x_scales, const void* w, const float* w_scales, const void* bias,
+                    void* y, int64_t M, int64_t N, int64_t K, int64_t x_stride, int64_t xs_stride_row,
+                    int64_t xs_stride_blk, int64_t w_stride, int64_t ws_stride_row, int64_t ws_stride_blk,
+                    int64_t y_stride, int out_dtype, int bias_dtype, int* status_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -53,6 +53,13 @@ SIGNATURES = {
     "qssm_rmsnorm_workspace_bytes": (_c_sz, [_c_i64]),
     "qssm_rmsnorm_fwd": (_c_int, [_c_vp] * 4 + [_c_i64] * 4 + [ctypes.c_float, _c_int, _c_vp]),
     "qssm_rmsnorm_bwd": (_c_int, [_c_vp] * 6 + [_c_vp, _c_sz] + [_c_i64] * 5 + [_c_int, _c_vp]),
+    "qssm_add_rmsnorm_workspace_bytes": (_c_sz, [_c_i64, _c_i64]),
+    "qssm_add_rmsnorm_fwd": (_c_int, [_c_vp] * 6 + [_c_i64] * 6 + [ctypes.c_float] + [_c_int] * 3 + [_c_vp]),
+    "qssm_add_rmsnorm_fp8": (_c_int, [_c_vp] * 6 + [_c_i64] * 8 + [ctypes.c_float] + [_c_int] * 3 + [_c_vp]),
+    "qssm_add_rmsnorm_bwd": (_c_int, [_c_vp] * 9 + [_c_sz] + [_c_i64] * 7 + [_c_int] * 3 + [_c_vp]),
+    "qssm_quant_fp8_rows": (_c_int, [_c_vp] * 3 + [_c_i64] * 6 + [_c_int, _c_vp]),
+    "qssm_quant_fp8_blocks": (_c_int, [_c_vp] * 3 + [_c_i64] * 6 + [_c_int, _c_vp]),
+    "qssm_matmul_fp8": (_c_int, [_c_vp] * 6 + [_c_i64] * 10 + [_c_int] * 2 + [_c_vp] * 2),
 }
 
 _lib = None
@@ -433,6 +440,86 @@ def rmsnorm_bwd(x, w, dy, rstd, dx, dw) -> None:
     if rc in (-3, -4):
         raise Unsupported(status_string(rc))
     _rc(rc, "qssm_rmsnorm_bwd")
+
+
+def _pitch(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.stride(0)
+
+
+def add_rmsnorm_fwd(x, res, w, y, h, rstd, eps: float) -> None:
+    """All but ``w`` and ``rstd`` are [rows, H] with a contiguous last axis; h = x + res, y = rms_norm(h) * w."""
+    dev = _require_cuda(x, res, w, y, h, rstd)
+    rows, H = x.shape
+    if _lib is None:
+        load()
+    with _on_device(dev):
+        rc = _lib.qssm_add_rmsnorm_fwd(_ptr(x), _ptr(res), _ptr(w), _ptr(y), _ptr(h), _ptr(rstd), rows, H, x.stride(0),
+                                       res.stride(0), y.stride(0), h.stride(0), eps, dtype_code(x.dtype),
+                                       dtype_code(res.dtype), dtype_code(w.dtype), _stream(dev))
+    if rc != 0:
+        _rc(rc, "qssm_add_rmsnorm_fwd")
+
+
+def add_rmsnorm_fp8(x, res, w, q, scales, h, eps: float) -> None:
+    """As ``add_rmsnorm_fwd`` with y left in e4m3 ``q`` [rows, H] and ``scales`` [rows, blocks]; res and h may be None."""
+    dev = _require_cuda(x, res, w, q, scales, h)
+    rows, H = x.shape
+    if _lib is None:
+        load()
+    with _on_device(dev):
+        code = dtype_code(x.dtype)
+        rc = _lib.qssm_add_rmsnorm_fp8(_ptr(x), _ptr(res), _ptr(w), _ptr(q), _ptr(scales), _ptr(h), rows, H, x.stride(0),
+                                       _pitch(res), q.stride(0), _pitch(h), scales.stride(0), scales.stride(1), eps,
+                                       code, code if res is None else dtype_code(res.dtype), dtype_code(w.dtype),
+                                       _stream(dev))
+    if rc != 0:
+        _rc(rc, "qssm_add_rmsnorm_fp8")
+
+
+def add_rmsnorm_bwd(h, w, dy, dh, rstd, dx, dres, dw) -> None:
+    """Gradients of ``add_rmsnorm_fwd``; dh, dx, dres may be None (not both of the last two)."""
+    dev = _require_cuda(h, w, dy, dh, rstd, dx, dres, dw)
+    rows, H = h.shape
+    if _lib is None:
+        load()
+    with _on_device(dev):
+        nbytes = int(_lib.qssm_add_rmsnorm_workspace_bytes(rows, H))
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        rc = _lib.qssm_add_rmsnorm_bwd(_ptr(h), _ptr(w), _ptr(dy), _ptr(dh), _ptr(rstd), _ptr(dx), _ptr(dres), _ptr(dw),
+                                       _ptr(ws), nbytes, rows, H, h.stride(0), dy.stride(0), _pitch(dh), _pitch(dx),
+                                       _pitch(dres), dtype_code(dy.dtype), dtype_code(h.dtype), dtype_code(w.dtype),
+                                       _stream(dev))
+    if rc != 0:
+        _rc(rc, "qssm_add_rmsnorm_bwd")
+
+
+def quant_fp8(x, q, scales, blocks: bool) -> None:
+    """e4m3 values ``q`` and ``scales`` of [rows, K] ``x``: per 128 of a row, or (``blocks``) per 128 x 128."""
+    dev = _require_cuda(x, q, scales)
+    rows, K = x.shape
+    if _lib is None:
+        load()
+    with _on_device(dev):
+        fn = _lib.qssm_quant_fp8_blocks if blocks else _lib.qssm_quant_fp8_rows
+        rc = fn(_ptr(x), _ptr(q), _ptr(scales), rows, K, x.stride(0), q.stride(0), scales.stride(0), scales.stride(1),
+                dtype_code(x.dtype), _stream(dev))
+    if rc != 0:
+        _rc(rc, "qssm_quant_fp8")
+
+
+def matmul_fp8(x, x_scales, w, w_scales, bias, y) -> None:
+    """y [M, N] = x [M, K] @ w [N, K]^T + bias on e4m3 operands whose rows start on 16-byte boundaries."""
+    dev = _require_cuda(x, x_scales, w, w_scales, bias, y)
+    M, K = x.shape
+    status = _begin(dev)
+    with _on_device(dev):
+        rc = _lib.qssm_matmul_fp8(x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), _ptr(bias),
+                                  y.data_ptr(), M, w.shape[0], K, x.stride(0), x_scales.stride(0), x_scales.stride(1),
+                                  w.stride(0), w_scales.stride(0), w_scales.stride(1), y.stride(0),
+                                  dtype_code(y.dtype), 0 if bias is None else dtype_code(bias.dtype), status,
+                                  _stream(dev))
+    if rc != 0:
+        _rc(rc, "qssm_matmul_fp8")
 
 
 MAX_PEERS, PEER_SLOTS = 16, 4

@@ -45,7 +45,6 @@
 #include <stdlib.h>
 #include <string.h>
 
-#include <mutex>
 #include <type_traits>
 #include <unordered_map>
 
@@ -53,6 +52,7 @@
 #include "qssm_bwd.cuh"
 #include "qssm_fwd.cuh"
 #include "qssm_gated.cuh"
+#include "qssm_host.cuh"
 #include "qssm_norm.cuh"
 #include "qssm_peer.cuh"
 
@@ -63,31 +63,6 @@ namespace {
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = []() -> EncodeTiledFn {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            return nullptr;
-        return reinterpret_cast<EncodeTiledFn>(p);
-    }();
-    return fn;
-}
-
-// Driver-API calls (tensor map encoding) need the primary context current on the calling thread;
-// a thread that has only inherited a device ordinal (e.g. an autograd worker) may not have one yet.
-void ensure_context() {
-    int dev = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
-}
-
-int dtype_size(int dt) { return dt == QSSM_F32 ? 4 : (dt == QSSM_F16 || dt == QSSM_BF16) ? 2 : 0; }
-
 CUtensorMapDataType tm_dtype(int dt) {
     return dt == QSSM_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                           : dt == QSSM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -214,28 +189,6 @@ int fill_desc(TensorDesc& td, const void* ptr, int dt, long long B, long long ro
     cache.map[slot] = td.map;
     cache.used[slot] = true;
     return 0;
-}
-
-constexpr int MAX_DEVICES = 64;
-
-int current_device() {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return 0;
-    return dev;
-}
-
-// SM count of the current device (looked up once per device ordinal).
-int sm_count() {
-    static int cached[MAX_DEVICES];
-    const int dev = current_device();
-    int n = __atomic_load_n(&cached[dev], __ATOMIC_RELAXED);
-    if (n <= 0) {
-        int v = 0;
-        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) v = 148;
-        n = v;
-        __atomic_store_n(&cached[dev], n, __ATOMIC_RELAXED);
-    }
-    return n;
 }
 
 // Launch shape of one call: channels per lane (V), rows per tile (TB), segments, ring depth.
@@ -391,34 +344,6 @@ int make_plan(Plan& pl, long long B, long long L, long long D, int n_seg, int* s
     pl.chains = B * n_seg * g.n_dtiles;
     g.n_chains = pl.chains;
     pl.grid = concurrent_chains(pl.chains, false);
-    return 0;
-}
-
-// Per kernel instantiation and device: the largest dynamic shared-memory size the function has been
-// opted into, and how many of its CTAs fit on an SM at a given size.  Both are asked of the runtime
-// once, not on every launch.
-struct KernelCache {
-    std::mutex mu;
-    std::unordered_map<unsigned long long, int> smem_set;   // (kernel, device) -> bytes
-    std::unordered_map<unsigned long long, int> per_sm;     // (kernel, device, smem, threads) -> CTAs per SM
-};
-KernelCache& kernel_cache() {
-    static KernelCache c;
-    return c;
-}
-inline unsigned long long kernel_key(const void* fn, int dev) {
-    return (unsigned long long)reinterpret_cast<uintptr_t>(fn) * 64ull + (unsigned long long)dev;
-}
-
-template <typename K> int ensure_smem(K kernel, int smem_bytes) {
-    KernelCache& kc = kernel_cache();
-    const unsigned long long key = kernel_key(reinterpret_cast<const void*>(kernel), current_device());
-    std::lock_guard<std::mutex> lock(kc.mu);
-    auto it = kc.smem_set.find(key);
-    if (it != kc.smem_set.end() && it->second >= smem_bytes) return 0;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
-    if (e != cudaSuccess) return (int)e;
-    kc.smem_set[key] = smem_bytes;
     return 0;
 }
 

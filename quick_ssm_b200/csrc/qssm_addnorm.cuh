@@ -1,0 +1,374 @@
+// Residual sum and RMS norm in one pass, forward (16/32-bit or e4m3 output) and backward.
+//
+//     h = x + residual (rounded to the residual's type)      r = 1 / sqrt(mean(h^2) + eps)      y = h * r * w
+//     d = dh + r * (w*dy) - h * r^3 * mean(h * w*dy)         dx = dres = d                      dw = sum over rows of dy * h * r
+//
+// h is rounded where it is stored, and the norm is taken of the stored values: the backward, and the next block,
+// see the h that the norm saw.  Sums, r and the arithmetic in between are fp32.
+//
+// All of it is bound by memory: forward 2 reads and 2 writes per element, backward 3 reads and one write (two if x
+// and the residual differ in type).  A row is owned by one warp or by the eight warps of a CTA and stays in
+// registers between its sum of squares and its output, so nothing is read twice; rows of more elements than the
+// registers hold are read again from the h that was just written (L1/L2).
+//
+// Columns are dealt to lanes in units: with V = 8 elements per access (16-bit data) a unit is 256 columns, lane l
+// owning columns 8l..8l+7; with V <= 4 it is 128 columns in 4/V accesses of V adjacent elements per lane.  Either way
+// a 128-column quantisation block lies in one access group of 16 or 32 lanes, and its largest magnitude is a shuffle
+// reduction.  V = 4 serves everything that has fp32 in it, V = 2 and 1 rows whose pitch or length allow no more.
+#pragma once
+#include "qssm_elem.cuh"
+
+namespace qssm {
+
+constexpr int ADDNORM_WARPS = 8;      // warps per CTA
+constexpr int ADDNORM_HELD = 32;      // elements of a row that a lane holds in registers
+constexpr int ADDNORM_CTAS = 4;       // upper bound of CTAs per SM in the backward (sizes its scratch)
+
+struct AddNormParams {
+    const void* x;
+    const void* res;     // NULL: h is x
+    const void* w;
+    void* y;             // forward: y, or the e4m3 values
+    void* h;             // forward: written if res != NULL; backward: read
+    float* rstd;         // forward: written if not NULL; backward: read
+    float* scales;       // fp8 output
+    const void* dy;      // backward
+    const void* dh;      // backward, may be NULL
+    void* dx;            // backward, may be NULL
+    void* dres;          // backward, may be NULL
+    float* dw_part;      // backward: [CTAs, H]
+    long long rows, x_stride, res_stride, y_stride, h_stride, dy_stride, dh_stride, dx_stride, dres_stride;
+    long long scale_row, scale_blk;
+    int H, w_dtype, w_vec;
+    float eps;
+};
+
+template <int V> struct Unit {
+    static constexpr int EPT = V == 8 ? 8 : 4;    // elements per lane
+    static constexpr int COLS = 32 * EPT;
+    static constexpr int ACC = EPT / V;           // accesses per lane
+    __device__ static __forceinline__ int col(int unit, int acc, int lane) {
+        return unit * COLS + acc * 32 * V + lane * V;
+    }
+};
+
+template <typename T, int V, int EPT>
+__device__ __forceinline__ void load_unit(const T* row, int unit, int lane, int H, float (&v)[EPT]) {
+#pragma unroll
+    for (int a = 0; a < Unit<V>::ACC; ++a) {
+        const int col = Unit<V>::col(unit, a, lane);
+        float t[V];
+        if (col < H) load_elems<T, V>(row + col, t);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[a * V + i] = col < H ? t[i] : 0.f;
+    }
+}
+template <typename T, int V, int EPT>
+__device__ __forceinline__ void store_unit(T* row, int unit, int lane, int H, const float (&v)[EPT]) {
+#pragma unroll
+    for (int a = 0; a < Unit<V>::ACC; ++a) {
+        const int col = Unit<V>::col(unit, a, lane);
+        float t[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = v[a * V + i];
+        if (col < H) store_elems<T, V>(row + col, t);
+    }
+}
+// The weight in its own type (0 fp32, 1 fp16, 2 bf16); 16-byte loads for fp32 weights that allow them.
+template <int V, int EPT>
+__device__ __forceinline__ void load_weight(const AddNormParams& p, int unit, int lane, float (&v)[EPT]) {
+#pragma unroll
+    for (int a = 0; a < Unit<V>::ACC; ++a) {
+        const int col = Unit<V>::col(unit, a, lane);
+        if constexpr (V >= 4) {
+            if (p.w_vec) {
+                float t[V];
+                if (col < p.H) load_elems<float, V>(static_cast<const float*>(p.w) + col, t);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[a * V + i] = col < p.H ? t[i] : 0.f;
+                continue;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float t = 0.f;
+            if (col + i < p.H) {
+                if (p.w_dtype == 0) t = static_cast<const float*>(p.w)[col + i];
+                else if (p.w_dtype == 1) t = to_f32(static_cast<const __half*>(p.w)[col + i]);
+                else t = to_f32(static_cast<const __nv_bfloat16*>(p.w)[col + i]);
+            }
+            v[a * V + i] = t;
+        }
+    }
+}
+// The sum over the row: one warp's, or the eight warps' partial sums added in warp order.  `red` alternates between
+// two sets of eight, so that one barrier per sum is enough.
+template <int WPR> __device__ __forceinline__ float sum_row(float v, float (*red)[ADDNORM_WARPS], int& turn) {
+    v = sum_warp(v);
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int k = 0; k < ADDNORM_WARPS; ++k) v += red[turn][k];
+        turn ^= 1;
+    }
+    return v;
+}
+
+// One unit of y, 16/32 bits, or quantised: the lanes of a 128-column block agree on its largest magnitude.
+template <typename TX, int V, bool FP8, int EPT>
+__device__ __forceinline__ void put_unit(const AddNormParams& p, long long row, int unit, int lane, const float (&y)[EPT]) {
+    if constexpr (!FP8) {
+        store_unit<TX, V>(static_cast<TX*>(p.y) + row * p.y_stride, unit, lane, p.H, y);
+    } else {
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) amax = max_nan(amax, fabsf(y[i]));
+        amax = max_lanes<V == 8 ? 16 : 32>(amax);
+        const float scale = fp8_scale(amax);
+        uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.y_stride;
+#pragma unroll
+        for (int a = 0; a < Unit<V>::ACC; ++a) {
+            const int col = Unit<V>::col(unit, a, lane);
+            float t[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[i] = y[a * V + i];
+            if (col < p.H) store_fp8<V>(q + col, t, scale);
+        }
+        const int first = Unit<V>::col(unit, 0, lane);
+        if ((lane & (V == 8 ? 15 : 31)) == 0 && first < p.H)
+            p.scales[row * p.scale_row + (long long)(first / FP8_BLOCK) * p.scale_blk] = scale;
+    }
+}
+
+// WPR: warps per row (1 or 8).  NU: units of a row held in registers by each of its warps, 0 for longer rows.
+template <typename TX, typename TR, int V, int WPR, int NU, bool FP8>
+__global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const AddNormParams p) {
+    constexpr int EPT = Unit<V>::EPT, N = NU > 0 ? NU : 1;
+    __shared__ float red[2][ADDNORM_WARPS];
+    int turn = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int wid = WPR > 1 ? warp : 0;
+    const long long first = WPR > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * ADDNORM_WARPS + warp;
+    const long long step = WPR > 1 ? (long long)gridDim.x : (long long)gridDim.x * ADDNORM_WARPS;
+    const int H = p.H;
+    const float inv_h = 1.f / (float)H;
+    float w[N][EPT];
+    if constexpr (NU > 0) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) load_weight<V>(p, u * WPR + wid, lane, w[u]);
+    }
+    for (long long row = first; row < p.rows; row += step) {
+        const TX* xr = static_cast<const TX*>(p.x) + row * p.x_stride;
+        const TR* rr = static_cast<const TR*>(p.res) + row * p.res_stride;
+        TR* hr = static_cast<TR*>(p.h) + row * p.h_stride;
+        float ss = 0.f;
+        if constexpr (NU > 0) {
+            float h[N][EPT];
+#pragma unroll
+            for (int u = 0; u < N; ++u) load_unit<TX, V>(xr, u * WPR + wid, lane, H, h[u]);
+            if (p.res != nullptr) {
+                float t[N][EPT];
+#pragma unroll
+                for (int u = 0; u < N; ++u) load_unit<TR, V>(rr, u * WPR + wid, lane, H, t[u]);
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+#pragma unroll
+                    for (int i = 0; i < EPT; ++i) h[u][i] = to_f32(from_f32<TR>(h[u][i] + t[u][i]));
+                    store_unit<TR, V>(hr, u * WPR + wid, lane, H, h[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) ss = fmaf(h[u][i], h[u][i], ss);
+            ss = sum_row<WPR>(ss, red, turn);
+            const float r = 1.f / sqrtf(ss * inv_h + p.eps);
+            if (p.rstd != nullptr && lane == 0 && wid == 0) p.rstd[row] = r;
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) h[u][i] *= w[u][i] * r;
+                put_unit<TX, V, FP8>(p, row, u * WPR + wid, lane, h[u]);
+            }
+        } else {
+            const int units = (H + Unit<V>::COLS - 1) / Unit<V>::COLS;
+            for (int u = wid; u < units; u += WPR) {
+                float h[EPT];
+                load_unit<TX, V>(xr, u, lane, H, h);
+                if (p.res != nullptr) {
+                    float t[EPT];
+                    load_unit<TR, V>(rr, u, lane, H, t);
+#pragma unroll
+                    for (int i = 0; i < EPT; ++i) h[i] = to_f32(from_f32<TR>(h[i] + t[i]));
+                    store_unit<TR, V>(hr, u, lane, H, h);
+                }
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) ss = fmaf(h[i], h[i], ss);
+            }
+            ss = sum_row<WPR>(ss, red, turn);
+            const float r = 1.f / sqrtf(ss * inv_h + p.eps);
+            if (p.rstd != nullptr && lane == 0 && wid == 0) p.rstd[row] = r;
+            for (int u = wid; u < units; u += WPR) {  // a lane reads back what it wrote itself
+                float h[EPT], wu[EPT];
+                if (p.res != nullptr) load_unit<TR, V>(hr, u, lane, H, h);
+                else load_unit<TX, V>(xr, u, lane, H, h);
+                load_weight<V>(p, u, lane, wu);
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) h[i] *= wu[i] * r;
+                put_unit<TX, V, FP8>(p, row, u, lane, h);
+            }
+        }
+    }
+}
+
+// Backward.  Each warp keeps the dw sums of its columns: in registers over all its rows (NU > 0), added up over the
+// CTA's warps in warp order at the end where every warp has rows of its own; for longer rows (eight warps each) in the
+// CTA's part of the scratch.
+template <typename TX, typename TR, int V, int WPR, int NU>
+__global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const AddNormParams p) {
+    constexpr int EPT = Unit<V>::EPT, N = NU > 0 ? NU : 1;
+    __shared__ float red[2][ADDNORM_WARPS];
+    extern __shared__ float dw_sum[];  // WPR == 1, NU > 0: H floats
+    int turn = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int wid = WPR > 1 ? warp : 0;
+    const long long first = WPR > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * ADDNORM_WARPS + warp;
+    const long long step = WPR > 1 ? (long long)gridDim.x : (long long)gridDim.x * ADDNORM_WARPS;
+    const int H = p.H;
+    const int units = (H + Unit<V>::COLS - 1) / Unit<V>::COLS;
+    const float inv_h = 1.f / (float)H;
+    float* part = p.dw_part + (long long)blockIdx.x * H;
+    float dw[N][EPT];
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) dw[u][i] = 0.f;
+    if constexpr (NU == 0) {
+        for (int u = wid; u < units; u += WPR) store_unit<float, V>(part, u, lane, H, dw[0]);
+    }
+    for (long long row = first; row < p.rows; row += step) {
+        const TR* hr = static_cast<const TR*>(p.h) + row * p.h_stride;
+        const TX* gr = static_cast<const TX*>(p.dy) + row * p.dy_stride;
+        const TR* er = static_cast<const TR*>(p.dh) + row * p.dh_stride;
+        TX* dxr = static_cast<TX*>(p.dx) + row * p.dx_stride;
+        TR* drr = static_cast<TR*>(p.dres) + row * p.dres_stride;
+        const float r = p.rstd[row];
+        float dot = 0.f;
+        if constexpr (NU > 0) {
+            float h[N][EPT], g[N][EPT], e[N][EPT];
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                load_unit<TR, V>(hr, u * WPR + wid, lane, H, h[u]);
+                load_unit<TX, V>(gr, u * WPR + wid, lane, H, g[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                if (p.dh != nullptr) load_unit<TR, V>(er, u * WPR + wid, lane, H, e[u]);
+                else {
+#pragma unroll
+                    for (int i = 0; i < EPT; ++i) e[u][i] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                float w[EPT];
+                load_weight<V>(p, u * WPR + wid, lane, w);
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) {
+                    dw[u][i] = fmaf(g[u][i] * r, h[u][i], dw[u][i]);
+                    g[u][i] *= w[i];
+                    dot = fmaf(h[u][i], g[u][i], dot);
+                }
+            }
+            dot = sum_row<WPR>(dot, red, turn);
+            const float k = dot * inv_h * r * r * r;
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) e[u][i] += fmaf(-h[u][i], k, r * g[u][i]);
+                if (p.dx != nullptr) store_unit<TX, V>(dxr, u * WPR + wid, lane, H, e[u]);
+                if (p.dres != nullptr) store_unit<TR, V>(drr, u * WPR + wid, lane, H, e[u]);
+            }
+        } else {
+            for (int u = wid; u < units; u += WPR) {
+                float h[EPT], g[EPT], w[EPT], s[EPT];
+                load_unit<TR, V>(hr, u, lane, H, h);
+                load_unit<TX, V>(gr, u, lane, H, g);
+                load_weight<V>(p, u, lane, w);
+                load_unit<float, V>(part, u, lane, H, s);
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) {
+                    dot = fmaf(h[i], g[i] * w[i], dot);
+                    s[i] = fmaf(g[i] * r, h[i], s[i]);
+                }
+                store_unit<float, V>(part, u, lane, H, s);
+            }
+            dot = sum_row<WPR>(dot, red, turn);
+            const float k = dot * inv_h * r * r * r;
+            for (int u = wid; u < units; u += WPR) {
+                float h[EPT], g[EPT], w[EPT], e[EPT];
+                load_unit<TR, V>(hr, u, lane, H, h);
+                load_unit<TX, V>(gr, u, lane, H, g);
+                load_weight<V>(p, u, lane, w);
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) e[i] = 0.f;
+                if (p.dh != nullptr) load_unit<TR, V>(er, u, lane, H, e);
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) e[i] += fmaf(-h[i], k, r * (w[i] * g[i]));
+                if (p.dx != nullptr) store_unit<TX, V>(dxr, u, lane, H, e);
+                if (p.dres != nullptr) store_unit<TR, V>(drr, u, lane, H, e);
+            }
+        }
+    }
+    if constexpr (NU > 0 && WPR > 1) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) store_unit<float, V>(part, u * WPR + wid, lane, H, dw[u]);
+    } else if constexpr (NU > 0) {
+        for (int k = 0; k < ADDNORM_WARPS; ++k) {
+            if (warp == k) {
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                    float s[EPT];
+#pragma unroll
+                    for (int i = 0; i < EPT; ++i) s[i] = 0.f;
+                    if (k > 0) load_unit<float, V>(dw_sum, u, lane, H, s);
+#pragma unroll
+                    for (int i = 0; i < EPT; ++i) s[i] += dw[u][i];
+                    store_unit<float, V>(k + 1 < ADDNORM_WARPS ? dw_sum : part, u, lane, H, s);
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// dw = the CTAs' partial sums, 32 columns a CTA: thread (tx, ty) adds rows ty, ty + 32, ..., four sums at a time, then
+// the 32 sums of a column are added in ty order.  The order does not depend on scheduling.
+template <typename TW>
+__global__ void __launch_bounds__(1024) addnorm_dw_kernel(const float* part, TW* dw, int n_part, int H) {
+    __shared__ float red[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int col = blockIdx.x * 32 + tx;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (col < H) {
+        const float* at = part + col;
+        int q = ty;
+        for (; q + 96 < n_part; q += 128) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += at[(long long)(q + 32 * i) * H];
+        }
+        for (; q < n_part; q += 32) s[0] += at[(long long)q * H];
+    }
+    red[ty][tx] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (ty == 0 && col < H) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t += red[k][tx];
+        dw[col] = from_f32<TW>(t);
+    }
+}
+
+}  // namespace qssm

@@ -1,0 +1,102 @@
+// Element access for the row kernels (residual norm, block quantisation): groups of 1 to 8 elements of fp32,
+// fp16 or bf16 as fp32 values, conversion to e4m3, warp reductions.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+namespace qssm {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <int BYTES> struct Word;
+template <> struct Word<2> { using type = uint16_t; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<16> { using type = uint4; };
+
+// V adjacent elements in one access (two 16-byte ones where they are longer than that).  The address is a multiple
+// of the access size.
+template <typename T, int V> __device__ __forceinline__ void load_elems(const T* p, float (&v)[V]) {
+    constexpr int BYTES = V * (int)sizeof(T);
+    if constexpr (BYTES > 16) {
+        static_assert(BYTES == 32, "at most two 16-byte accesses");
+        float lo[V / 2], hi[V / 2];
+        load_elems<T, V / 2>(p, lo);
+        load_elems<T, V / 2>(p + V / 2, hi);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) { v[i] = lo[i]; v[V / 2 + i] = hi[i]; }
+    } else {
+        union { typename Word<BYTES>::type w; T e[V]; } u;
+        u.w = *reinterpret_cast<const typename Word<BYTES>::type*>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = to_f32(u.e[i]);
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void store_elems(T* p, const float (&v)[V]) {
+    constexpr int BYTES = V * (int)sizeof(T);
+    if constexpr (BYTES > 16) {
+        float lo[V / 2], hi[V / 2];
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) { lo[i] = v[i]; hi[i] = v[V / 2 + i]; }
+        store_elems<T, V / 2>(p, lo);
+        store_elems<T, V / 2>(p + V / 2, hi);
+    } else {
+        union U { typename Word<BYTES>::type w; T e[V]; __device__ U() {} } u;
+#pragma unroll
+        for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
+        *reinterpret_cast<typename Word<BYTES>::type*>(p) = u.w;
+    }
+}
+
+__device__ __forceinline__ float sum_warp(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// fmaxf drops a NaN; a block that holds one has to end up NaN as a whole.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+template <int LANES> __device__ __forceinline__ float max_lanes(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// Quantisation of a block: scale = max(amax, 2^-100) / 448 (448 is e4m3's largest value; the floor keeps the scale a
+// normal number for blocks of zeros), value = e4m3(v / scale), nearest even.  An infinity in the block makes the scale
+// infinite and its own value NaN, a NaN makes the scale NaN: what is computed from such a block is NaN.
+constexpr float FP8_MAX = 448.f;
+constexpr float FP8_AMAX_FLOOR = 7.888609052210118e-31f;  // 2^-100
+constexpr int FP8_BLOCK = 128;
+
+__device__ __forceinline__ float fp8_scale(float amax) { return max_nan(amax, FP8_AMAX_FLOOR) / FP8_MAX; }
+
+template <int V> __device__ __forceinline__ void store_fp8(uint8_t* p, const float (&v)[V], float scale) {
+    float q[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[i] = v[i] / scale;
+    if constexpr (V == 1) {
+        *p = __nv_cvt_float_to_fp8(q[0], __NV_SATFINITE, __NV_E4M3);
+    } else {
+        union { typename Word<V>::type w; uint16_t h[V / 2]; } u;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+            u.h[i] = __nv_cvt_float2_to_fp8x2(make_float2(q[2 * i], q[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+        *reinterpret_cast<typename Word<V>::type*>(p) = u.w;
+    }
+}
+
+}  // namespace qssm

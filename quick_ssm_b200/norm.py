@@ -6,12 +6,20 @@
 and dy and writes dx; dw is summed in a fixed order (no atomics).  Shapes the kernels cannot take
 (last axis not a multiple of 4, unaligned views) are composed from torch operations on the same
 device; CPU tensors raise.
+
+``add_rms_norm`` and ``add_rms_norm_fp8`` put the residual's addition in front, as it stands between
+two blocks of a stack: ``h = x + residual`` is written once and its norm leaves the same kernel, in
+x's type with a backward pass (training), or in e4m3 with a scale for each 128 values (serving, the
+operand of ``fp8.matmul_fp8``).  They take any row length, pitch and alignment.
 """
 from __future__ import annotations
+
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
+from .fp8 import Fp8Rows, rows_2d, rows_like
 
 
 def _composed(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
@@ -53,3 +61,82 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.
     if H % 4 != 0 or x.numel() == 0 or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         return _composed(x, weight, eps)
     return _RMSNormFunction.apply(x, weight, eps)
+
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _check_add(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, name: str) -> None:
+    if x.device.type != "cuda":
+        raise RuntimeError(f"{name} needs CUDA tensors; there is no CPU path")
+    if x.dtype not in _FLOATS or weight.dtype not in _FLOATS:
+        raise TypeError(f"{name} takes float32, float16 and bfloat16; got {x.dtype} with a weight in {weight.dtype}")
+    if x.dim() < 1 or weight.shape != x.shape[-1:]:
+        raise ValueError("weight must have the size of the last axis of x")
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"residual is {tuple(residual.shape)}, x is {tuple(x.shape)}")
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"residual must be in x's type or in float32; got {residual.dtype} with x in {x.dtype}")
+
+
+class _AddRMSNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        x2, r2, w = rows_2d(x), rows_2d(residual), weight.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        rstd = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
+        _lib.add_rmsnorm_fwd(x2, r2, w, rows_2d(y), rows_2d(h), rstd, eps)
+        ctx.save_for_backward(h, w, rstd)
+        ctx.set_materialize_grads(False)
+        ctx.x_dtype = x.dtype
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        h, w, rstd = ctx.saved_tensors
+        need_x, need_r, need_w, _ = ctx.needs_input_grad
+        shape, xd, rd = h.shape, ctx.x_dtype, h.dtype
+        h = rows_2d(h)
+        if dy is None:  # only h was used: its gradient passes through
+            dx = dh.to(xd) if need_x and dh is not None else None
+            return dx, dh if need_r else None, None, None
+        dev = h.device
+        dx = torch.empty(h.shape, dtype=xd, device=dev) if need_x or rd == xd else None
+        dres = torch.empty(h.shape, dtype=rd, device=dev) if rd != xd and (need_r or dx is None) else None
+        dw = torch.empty(w.shape, dtype=w.dtype, device=dev)
+        _lib.add_rmsnorm_bwd(h, w, rows_2d(dy.to(xd)), None if dh is None else rows_2d(dh.to(rd)), rstd, dx, dres, dw)
+        gx = dx.view(shape) if need_x else None
+        gr = (dx if rd == xd else dres).view(shape) if need_r else None
+        return gx, gr, dw if need_w else None, None
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                 eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``h = x + residual`` and ``y = h * weight / sqrt(mean(h^2, -1) + eps)``; returns ``(y, h)``.
+
+    ``x``: ``[..., H]`` fp32, fp16 or bf16; ``residual``: the same shape, in x's type or in fp32 (a 32-bit residual
+    stream under 16-bit branches).  ``y`` has x's type, ``h`` the residual's; the norm is that of ``h`` as stored.
+    Differentiable in x, residual and weight."""
+    _check_add(x, residual, weight, "add_rms_norm")
+    if residual is None:
+        raise ValueError("add_rms_norm needs a residual; rms_norm is the norm alone")
+    return _AddRMSNormFunction.apply(x, residual, weight, float(eps))
+
+
+@torch.no_grad()
+def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
+                     eps: float = 1e-5) -> Tuple[Fp8Rows, torch.Tensor]:
+    """The sum and norm of ``add_rms_norm`` with y quantised for ``fp8.matmul_fp8``; returns ``(y, h)``.
+
+    The scales are taken from y in 32 bits: it is rounded once, to e4m3.  ``residual=None`` (the first block of a
+    stack): h is x itself.  Serving only, no gradient."""
+    _check_add(x, residual, weight, "add_rms_norm_fp8")
+    x2 = rows_2d(x)
+    r2 = None if residual is None else rows_2d(residual)
+    h = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    q = rows_like(x2)
+    _lib.add_rmsnorm_fp8(x2, r2, weight.contiguous(), q.values, q.scales, None if residual is None else rows_2d(h), float(eps))
+    return q.view_as_rows_of(x.shape), h
