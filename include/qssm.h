@@ -374,8 +374,8 @@ int qssm_quant_fp8_blocks(const void* w, void* q, float* scales, int64_t N, int6
  *     y[m, n] = bias[n] + sum_b x_scales[m, b] * w_scales[n/128, b] * sum_{k in block b} x[m, k] * w[n, k]
  * x [M, K], w [N, K]: e4m3, rows x_stride / w_stride bytes apart; both strides and both bases multiples of 16
  * (QSSM_E_STRIDE otherwise).  Scales fp32 with strides of their own.  bias: N elements of bias_dtype, or NULL.
- * y: out_dtype (any of the three), rows y_stride elements apart.  Sums in fp32, one rounding at the end.  K = 0 gives
- * the bias.  status_word as above (an expired wait on a bulk copy).
+ * y: out_dtype (any of the three), rows y_stride elements apart.  Sums in fp32, one rounding at the end.  K = 0 is
+ * refused (QSSM_E_SHAPE).  status_word as above (an expired wait on a bulk copy).
  */
 int qssm_matmul_fp8(const void* x, const float* x_scales, const void* w, const float* w_scales, const void* bias,
                     void* y, int64_t M, int64_t N, int64_t K, int64_t x_stride, int64_t xs_stride_row,

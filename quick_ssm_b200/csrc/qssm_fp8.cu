@@ -30,6 +30,84 @@ int quant_check(const void* x, const void* q, const void* scales, long long rows
     return 0;
 }
 
+// e4m3 [rows, K] as the product's copies see it: boxes of 128 bytes of k and `box_rows` rows in the 128-byte swizzle,
+// zeros outside.  Each host thread keeps the maps it encoded last, as the scan does.
+int fp8_map(CUtensorMap& map, const void* ptr, long long rows, long long K, long long stride, int box_rows) {
+    struct Key {
+        const void* ptr;
+        long long rows, K, stride, box;
+        bool operator==(const Key& o) const {
+            return ptr == o.ptr && rows == o.rows && K == o.K && stride == o.stride && box == o.box;
+        }
+    };
+    struct Entry { Key key; CUtensorMap map; };
+    static thread_local Entry cache[64];
+    static thread_local bool have_context = false;
+    const Key key{ptr, rows, K, stride, box_rows};
+    const unsigned long long hash = ((unsigned long long)reinterpret_cast<uintptr_t>(ptr) + 64ull * box_rows + rows) * 0x9E3779B97F4A7C15ull;
+    Entry& e = cache[hash >> 58];
+    if (e.key == key) {
+        map = e.map;
+        return 0;
+    }
+    if (!have_context) {
+        ensure_context();
+        have_context = true;
+    }
+    EncodeTiledFn enc = encode_fn();
+    if (enc == nullptr) return QSSM_E_DRIVER;
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+    cuuint32_t box[2] = {(cuuint32_t)MM_TILE_K, (cuuint32_t)box_rows}, estr[2] = {1u, 1u};
+    if (enc(&e.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        e.key.ptr = nullptr;
+        return QSSM_E_STRIDE;
+    }
+    e.key = key;
+    map = e.map;
+    return 0;
+}
+
+struct MatmulPlan {
+    int T;  // rows per tile of the few-rows kernel; 0: the many-rows kernel
+    int S;  // CTAs that share a tile's k
+    int x_box, w_box;
+};
+
+MatmulPlan plan_matmul(long long M, long long N, int n_kb) {
+    const long long sms = sm_count();
+    const long long big = ((M + MMR_M - 1) / MMR_M) * ((N + MMR_N - 1) / MMR_N);
+    if (M > 64 && big >= sms) return {0, 1, MMR_M, MMR_N};
+    const int T = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const long long tiles = ((N + 127) / 128) * ((M + T - 1) / T);
+    int S = 1;
+    while (S < 8 && tiles * S * 2 <= 2 * sms && n_kb >= 4 * S) S *= 2;
+    return {T, S, T, 128};
+}
+
+template <typename OUT, int T> int launch_few(const MatmulParams& p, int S, cudaStream_t stream) {
+    auto kernel = matmul_fp8_few_kernel<OUT, T>;
+    const int rc = ensure_smem(kernel, Few<T>::SMEM);
+    if (rc) return rc;
+    const long long gx = (long long)((p.N + 127) / 128) * S, gy = (p.M + T - 1) / T;
+    if (gy > 65535 || gx >= (1ll << 31)) return QSSM_E_SHAPE;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)gx, (unsigned)gy);
+    cfg.blockDim = dim3(MMF_THREADS);
+    cfg.dynamicSmemBytes = Few<T>::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)S;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, p, S);
+}
+
 }  // namespace
 
 extern "C" {
@@ -72,28 +150,46 @@ int qssm_quant_fp8_blocks(const void* w, void* q, float* scales, int64_t N, int6
 int qssm_matmul_fp8(const void* x, const float* x_scales, const void* w, const float* w_scales, const void* bias,
                     void* y, int64_t M, int64_t N, int64_t K, int64_t x_stride, int64_t xs_stride_row,
                     int64_t xs_stride_blk, int64_t w_stride, int64_t ws_stride_row, int64_t ws_stride_blk,
-                    int64_t y_stride, int out_dtype, int bias_dtype, int* status_word, void* stream) {
+                    int64_t y_stride, int out_dtype, int bias_dtype, int* status_word, void* stream_v) {
     if (dtype_size(out_dtype) == 0 || (bias != nullptr && dtype_size(bias_dtype) == 0)) return QSSM_E_DTYPE;
     if (M < 0 || N < 0 || K < 0 || M >= (1ll << 31) - 256 || N >= (1ll << 31) - 256 || K >= (1ll << 30)) return QSSM_E_SHAPE;
     if (M == 0 || N == 0) return 0;
-    if (y == nullptr || (K > 0 && (x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr)))
-        return QSSM_E_NULL;
-    if (y_stride < N || (K > 0 && (x_stride < K || w_stride < K || !fits(x, x_stride, 16, 1) || !fits(w, w_stride, 16, 1))))
+    if (K == 0) return QSSM_E_SHAPE;
+    if (y == nullptr || x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr) return QSSM_E_NULL;
+    if (y_stride < N || x_stride < K || w_stride < K || !fits(x, x_stride, 16, 1) || !fits(w, w_stride, 16, 1))
         return QSSM_E_STRIDE;
     MatmulParams p;
     memset(&p, 0, sizeof(p));
-    p.x = static_cast<const uint8_t*>(x); p.w = static_cast<const uint8_t*>(w);
     p.x_scales = x_scales; p.w_scales = w_scales; p.bias = bias; p.y = y;
-    p.M = M; p.N = N; p.K = K;
-    p.x_stride = x_stride; p.xs_row = xs_stride_row; p.xs_blk = xs_stride_blk;
-    p.w_stride = w_stride; p.ws_row = ws_stride_row; p.ws_blk = ws_stride_blk; p.y_stride = y_stride;
+    p.M = (int)M; p.N = (int)N; p.K = (int)K; p.n_kb = (int)((K + MM_TILE_K - 1) / MM_TILE_K);
+    p.xs_row = xs_stride_row; p.xs_blk = xs_stride_blk; p.ws_row = ws_stride_row; p.ws_blk = ws_stride_blk;
+    p.y_stride = y_stride;
     p.bias_dtype = bias_dtype; p.status = status_word;
+    const int es = dtype_size(out_dtype);
+    p.y_vec = fits(y, y_stride, 16, es);
+    const MatmulPlan plan = plan_matmul(M, N, p.n_kb);
+    int rc;
+    if ((rc = fp8_map(p.x_map, x, M, K, x_stride, plan.x_box)) || (rc = fp8_map(p.w_map, w, N, K, w_stride, plan.w_box)))
+        return rc;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     return with_type(out_dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16));
-        if (grid.y > 65535u) return QSSM_E_SHAPE;
-        matmul_fp8_plain_kernel<T><<<grid, dim3(16, 16), 0, static_cast<cudaStream_t>(stream)>>>(p);
-        return (int)cudaGetLastError();
+        if (plan.T == 0) {
+            p.m_tiles = (int)((M + MMR_M - 1) / MMR_M);
+            p.n_tiles = (int)((N + MMR_N - 1) / MMR_N);
+            const long long tiles = (long long)p.m_tiles * p.n_tiles;
+            if (tiles >= (1ll << 31) - 1024) return QSSM_E_SHAPE;
+            if ((rc = ensure_smem(matmul_fp8_rows_kernel<T>, MMR_SMEM))) return rc;
+            const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
+            matmul_fp8_rows_kernel<T><<<grid, MMR_THREADS, MMR_SMEM, stream>>>(p);
+            return (int)cudaGetLastError();
+        }
+        switch (plan.T) {
+            case 16: return launch_few<T, 16>(p, plan.S, stream);
+            case 32: return launch_few<T, 32>(p, plan.S, stream);
+            case 64: return launch_few<T, 64>(p, plan.S, stream);
+            default: return launch_few<T, 128>(p, plan.S, stream);
+        }
     });
 }
 

@@ -2,57 +2,357 @@
 //
 //     y[m, n] = bias[n] + sum over blocks kb of  sx[m, kb] * sw[n / 128, kb] * sum over k in kb of  x[m, k] * w[n, k]
 //
-// Inner sums and the sum over blocks are fp32; the result is rounded once.
+// The inner sum of a block is four tcgen05 products of 32 along k into tensor memory; the scales are not powers of
+// two in general, so each block's result is read back (tcgen05.ld) and added to fp32 sums in registers with its scale
+// while the tensor cores work on the next block in the other buffer.  Inner sums and the sum over blocks are fp32;
+// the result is rounded once.
+//
+// Roles: one thread issues the bulk copies (TMA, 128-byte swizzle, zero fill behind the last row and the last k), one
+// the products, the other warps own the sums.  Every wait on a barrier gives up after two seconds and reports
+// QSSM_S_TMA_TIMEOUT; the CTA then still waits for its own copies and products and frees its tensor memory.
 #pragma once
 #include "qssm_elem.cuh"
+#include "qssm_tc.cuh"
 
 namespace qssm {
 
 struct MatmulParams {
-    const uint8_t* x;       // [M, K] e4m3, rows x_stride bytes apart
-    const uint8_t* w;       // [N, K] e4m3
+    CUtensorMap x_map, w_map;
     const float* x_scales;  // [M, K/128]
     const float* w_scales;  // [N/128, K/128]
     const void* bias;       // [N] or NULL
     void* y;                // [M, N]
-    long long M, N, K, x_stride, xs_row, xs_blk, w_stride, ws_row, ws_blk, y_stride;
-    int bias_dtype;
+    long long xs_row, xs_blk, ws_row, ws_blk, y_stride;
+    int M, N, K, n_kb;      // n_kb: blocks of 128 along k
+    int m_tiles, n_tiles;
+    int bias_dtype, y_vec;  // y_vec: rows of y start on 16-byte boundaries
     int* status;
 };
 
-__device__ __forceinline__ float e4m3_to_f32(uint8_t v) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
-}
-__device__ __forceinline__ float load_bias(const MatmulParams& p, long long n) {
-    if (p.bias == nullptr) return 0.f;
+constexpr int MM_TIMEOUT = 10001;  // QSSM_S_TMA_TIMEOUT
+constexpr int MM_TILE_K = 128;
+
+__device__ __forceinline__ float load_bias(const MatmulParams& p, int n) {
+    if (p.bias == nullptr || n >= p.N) return 0.f;
     if (p.bias_dtype == 0) return static_cast<const float*>(p.bias)[n];
     if (p.bias_dtype == 1) return to_f32(static_cast<const __half*>(p.bias)[n]);
     return to_f32(static_cast<const __nv_bfloat16*>(p.bias)[n]);
 }
+__device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 
-// One thread per output, operands of a 16 x 16 tile through shared memory.
-template <typename T> __global__ void __launch_bounds__(256) matmul_fp8_plain_kernel(const MatmulParams p) {
-    __shared__ float xs[16][129], ws[16][129];
-    const int tx = threadIdx.x, ty = threadIdx.y;
-    const long long m0 = (long long)blockIdx.y * 16, n0 = (long long)blockIdx.x * 16;
-    const long long m = m0 + ty, n = n0 + tx;
-    float sum = 0.f;
-    for (long long k0 = 0; k0 < p.K; k0 += 128) {
-        for (int i = ty * 16 + tx; i < 16 * 128; i += 256) {
-            const int r = i >> 7, c = i & 127;
-            xs[r][c] = m0 + r < p.M && k0 + c < p.K ? e4m3_to_f32(p.x[(m0 + r) * p.x_stride + k0 + c]) : 0.f;
-            ws[r][c] = n0 + r < p.N && k0 + c < p.K ? e4m3_to_f32(p.w[(n0 + r) * p.w_stride + k0 + c]) : 0.f;
-        }
-        __syncthreads();
-        float t = 0.f;
-        for (int c = 0; c < 128; ++c) t = fmaf(xs[ty][c], ws[tx][c], t);
-        if (m < p.M && n < p.N) {
-            const long long kb = k0 / 128;
-            sum = fmaf(t, p.x_scales[m * p.xs_row + kb * p.xs_blk] * p.w_scales[(n / 128) * p.ws_row + kb * p.ws_blk], sum);
-        }
-        __syncthreads();
+// ---------------------------------------------------------------------------------------------
+// Many rows: tiles of 128 rows x 256 columns, a persistent CTA per SM.  Lane = row: a thread owns one row's sums of
+// 128 columns, and both scales of a block are one factor for all of them.
+// ---------------------------------------------------------------------------------------------
+constexpr int MMR_M = 128, MMR_N = 256, MMR_STAGES = 4;
+constexpr int MMR_A = MMR_M * MM_TILE_K, MMR_STAGE = MMR_A + MMR_N * MM_TILE_K;
+constexpr int MMR_THREADS = 320;  // warps 0-7 sums, 8 copies, 9 products
+constexpr int MMR_SMEM = MMR_STAGES * MMR_STAGE + 8 * 128 * 4 + 256 + 1024;
+
+template <typename T> __global__ void __launch_bounds__(MMR_THREADS, 1) matmul_fp8_rows_kernel(const __grid_constant__ MatmulParams p) {
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t base = smem_u32(smem);
+    float* bias_at = reinterpret_cast<float*>(smem + MMR_STAGES * MMR_STAGE);
+    const uint32_t bars = base + MMR_STAGES * MMR_STAGE + 8 * 128 * 4;
+    const uint32_t full = bars, empty = full + 8 * MMR_STAGES, done = empty + 8 * MMR_STAGES, taken = done + 16, last = taken + 16;
+    volatile uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + (last + 8 - base));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, 8); }
+        mbar_init(last, 1);
+        fence_barrier_init();
     }
-    if (m < p.M && n < p.N) static_cast<T*>(p.y)[m * p.y_stride + n] = from_f32<T>(sum + load_bias(p, n));
+    if (warp == 9) tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_at)), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_at;
+    const int tiles = p.m_tiles * p.n_tiles;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            prefetch_map(&p.x_map);
+            prefetch_map(&p.w_map);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+                const int m0 = (t % p.m_tiles) * MMR_M, n0 = (t / p.m_tiles) * MMR_N;
+                for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
+                    const uint32_t s = it % MMR_STAGES, round = it / MMR_STAGES;
+                    if (round > 0 && !mbar_wait_limit(empty + 8 * s, (round - 1) & 1)) { ok = false; break; }
+                    mbar_expect_tx(full + 8 * s, MMR_STAGE);
+                    tma_load_2d(base + s * MMR_STAGE, &p.x_map, full + 8 * s, kb * MM_TILE_K, m0);
+                    tma_load_2d(base + s * MMR_STAGE + MMR_A, &p.w_map, full + 8 * s, kb * MM_TILE_K, n0);
+                }
+            }
+            // no copy outlives the CTA
+            const uint32_t left = it < (uint32_t)MMR_STAGES ? it : (uint32_t)MMR_STAGES;
+            for (uint32_t i = it - left; i < it; ++i) ok &= mbar_wait_limit(full + 8 * (i % MMR_STAGES), (i / MMR_STAGES) & 1);
+            if (!ok && p.status != nullptr) *p.status = MM_TIMEOUT;
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = fp8_idesc(MMR_M, MMR_N);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+                for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
+                    const uint32_t s = it % MMR_STAGES, b = it & 1;
+                    if (it >= 2 && !mbar_wait_limit(taken + 8 * b, ((it >> 1) - 1) & 1)) { ok = false; break; }
+                    if (!mbar_wait_limit(full + 8 * s, (it / MMR_STAGES) & 1)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t a = smem_operand(base + s * MMR_STAGE), w = smem_operand(base + s * MMR_STAGE + MMR_A);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc_mma_fp8(tmem + b * MMR_N, a + 2 * k, w + 2 * k, idesc, k > 0);
+                    tc_commit(empty + 8 * s);
+                    tc_commit(done + 8 * b);
+                }
+            }
+            tc_commit(last);  // no product outlives the CTA
+            ok &= mbar_wait_limit(last, 0);
+            if (!ok && p.status != nullptr) *p.status = MM_TIMEOUT;
+        }
+    } else {
+        const int half = warp >> 2;
+        const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
+        float* my_bias = bias_at + warp * 128;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            const int m = (t % p.m_tiles) * MMR_M + (warp & 3) * 32 + lane, n0 = (t / p.m_tiles) * MMR_N + half * 128;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) my_bias[i * 32 + lane] = load_bias(p, n0 + i * 32 + lane);
+            __syncwarp();
+            float2 acc[64];  // the sums start from the bias
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const float4 v = *reinterpret_cast<const float4*>(my_bias + 4 * j);
+                acc[2 * j] = make_float2(v.x, v.y);
+                acc[2 * j + 1] = make_float2(v.z, v.w);
+            }
+            const float* xs = p.x_scales + (long long)(m < p.M ? m : 0) * p.xs_row;
+            const float* ws = p.w_scales + (long long)(n0 < p.N ? n0 / 128 : 0) * p.ws_row;
+            // scales two blocks ahead of their use
+            float s0 = xs[0] * ws[0], s1 = p.n_kb > 1 ? xs[p.xs_blk] * ws[p.ws_blk] : 0.f;
+            for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
+                float xa = 0.f, wa = 0.f;
+                if (kb + 2 < p.n_kb) { xa = xs[(kb + 2) * p.xs_blk]; wa = ws[(kb + 2) * p.ws_blk]; }
+                const uint32_t b = it & 1;
+                if (!mbar_wait_limit(done + 8 * b, (it >> 1) & 1)) { ok = false; break; }
+                tc_fence_after();
+                const float2 s = make_float2(s0, s0);
+                uint32_t r[2][32];
+                tmem_ld<32>(at + b * MMR_N, r[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tc_wait_ld(r[c & 1]);
+                    if (c < 3) tmem_ld<32>(at + b * MMR_N + 32 * (c + 1), r[(c + 1) & 1]);
+                    else {  // all read: the buffer may be written again
+                        tc_fence_before();
+                        if (lane == 0) mbar_arrive(taken + 8 * b);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) fma_pair(acc[16 * c + j], as_pair(r[c & 1][2 * j], r[c & 1][2 * j + 1]), s);
+                }
+                s0 = s1;
+                s1 = xa * wa;
+            }
+            if (!ok) break;
+            if (m < p.M) {
+                T* yr = static_cast<T*>(p.y) + (long long)m * p.y_stride + n0;
+                constexpr int V = 16 / sizeof(T);
+#pragma unroll
+                for (int j = 0; j < 128; j += V) {
+                    float v[V];
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) { v[i] = acc[(j + i) / 2].x; v[i + 1] = acc[(j + i) / 2].y; }
+                    if (p.y_vec && n0 + j + V <= p.N) store_elems<T, V>(yr + j, v);
+                    else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            if (n0 + j + i < p.N) yr[j + i] = from_f32<T>(v[i]);
+                    }
+                }
+            }
+        }
+        if (!ok && lane == 0 && p.status != nullptr) *p.status = MM_TIMEOUT;
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_free(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few rows: the weight is the first operand.  Tiles of 128 columns of y x T rows (T = 16 to 128), lane = column, so
+// the weight's rows fill the tensor cores' 128 lanes however few rows there are, and k is cut over the S CTAs of a
+// cluster, whose sums are added in rank order through distributed shared memory (each CTA adds T / S of the rows).
+// ---------------------------------------------------------------------------------------------
+template <int T> struct Few {
+    static constexpr int A = 128 * MM_TILE_K, STAGE = A + T * MM_TILE_K;
+    static constexpr int STAGES = T <= 32 ? 5 : T == 64 ? 4 : 3;   // two CTAs on an SM
+    static constexpr int BUFS = 2;
+    static constexpr uint32_t TMEM = BUFS * T < 32 ? 32 : BUFS * T;
+    static constexpr int SCALES = 4 * 2 * T * 4;                    // per warp: two sets of T factors
+    static constexpr int SMEM = STAGES * STAGE + SCALES + 256 + 1024;
+    static_assert(STAGES * STAGE >= T * 128 * 4, "the sums are handed over in the stages' memory");
+};
+constexpr int MMF_THREADS = 192;  // warps 0-3 sums, 4 copies, 5 products
+
+template <typename OUT, int T> __global__ void __launch_bounds__(MMF_THREADS, 2) matmul_fp8_few_kernel(const __grid_constant__ MatmulParams p, int S) {
+    using C = Few<T>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t base = smem_u32(smem);
+    const uint32_t bars = base + C::STAGES * C::STAGE + C::SCALES;
+    const uint32_t full = bars, empty = full + 8 * C::STAGES, done = empty + 8 * C::STAGES, taken = done + 8 * C::BUFS,
+                   last = taken + 8 * C::BUFS;
+    volatile uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + (last + 8 - base));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (int b = 0; b < C::BUFS; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, 4); }
+        mbar_init(last, 1);
+        fence_barrier_init();
+    }
+    if (warp == 5) tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_at)), C::TMEM);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_at;
+    const int rank = S > 1 ? (int)cluster_rank() : 0;
+    const int n0 = ((int)blockIdx.x / S) * 128, m0 = (int)blockIdx.y * T;
+    const int kb0 = (int)((long long)p.n_kb * rank / S), kb1 = (int)((long long)p.n_kb * (rank + 1) / S);
+    const int n = n0 + (warp & 3) * 32 + lane;
+    float2 acc[T / 2];
+
+    if (warp == 4) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const uint32_t s = it % C::STAGES, round = it / C::STAGES;
+                if (round > 0 && !mbar_wait_limit(empty + 8 * s, (round - 1) & 1)) { ok = false; break; }
+                mbar_expect_tx(full + 8 * s, C::STAGE);
+                tma_load_2d(base + s * C::STAGE, &p.w_map, full + 8 * s, kb * MM_TILE_K, n0);
+                tma_load_2d(base + s * C::STAGE + C::A, &p.x_map, full + 8 * s, kb * MM_TILE_K, m0);
+            }
+            const uint32_t left = it < (uint32_t)C::STAGES ? it : (uint32_t)C::STAGES;
+            for (uint32_t i = it - left; i < it; ++i) ok &= mbar_wait_limit(full + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
+            if (!ok && p.status != nullptr) *p.status = MM_TIMEOUT;
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = fp8_idesc(128, T);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const uint32_t s = it % C::STAGES, b = it % C::BUFS;
+                if (it >= (uint32_t)C::BUFS && !mbar_wait_limit(taken + 8 * b, (it / C::BUFS - 1) & 1)) { ok = false; break; }
+                if (!mbar_wait_limit(full + 8 * s, (it / C::STAGES) & 1)) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t w = smem_operand(base + s * C::STAGE), x = smem_operand(base + s * C::STAGE + C::A);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc_mma_fp8(tmem + b * T, w + 2 * k, x + 2 * k, idesc, k > 0);
+                tc_commit(empty + 8 * s);
+                tc_commit(done + 8 * b);
+            }
+            tc_commit(last);
+            ok &= mbar_wait_limit(last, 0);
+            if (!ok && p.status != nullptr) *p.status = MM_TIMEOUT;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < T / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+        const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16);
+        constexpr int PER = (T + 31) / 32;  // rows whose factor a lane prepares
+        float* factors = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE) + warp * 2 * T;
+        const float* ws = p.w_scales + (long long)(n0 / 128) * p.ws_row;
+        const float* xs[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int m = m0 + i * 32 + lane;
+            xs[i] = p.x_scales + (long long)(m < p.M ? m : 0) * p.xs_row;
+        }
+        float next[PER], wnext = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) next[i] = 0.f;
+        if (kb0 < kb1) {
+            wnext = ws[kb0 * p.ws_blk];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) next[i] = xs[i][kb0 * p.xs_blk];
+        }
+        uint32_t it = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            float* f = factors + (it & 1) * T;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (i * 32 + lane < T) f[i * 32 + lane] = next[i] * wnext;
+            __syncwarp();
+            if (kb + 1 < kb1) {
+                wnext = ws[(kb + 1) * p.ws_blk];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) next[i] = xs[i][(kb + 1) * p.xs_blk];
+            }
+            const uint32_t b = it % C::BUFS;
+            if (!mbar_wait_limit(done + 8 * b, (it / C::BUFS) & 1)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t r[2][16];
+            tmem_ld<16>(at + b * T, r[0]);
+#pragma unroll
+            for (int c = 0; c < T / 16; ++c) {
+                tc_wait_ld(r[c & 1]);
+                if (c + 1 < T / 16) tmem_ld<16>(at + b * T + 16 * (c + 1), r[(c + 1) & 1]);
+                else {
+                    tc_fence_before();
+                    if (lane == 0) mbar_arrive(taken + 8 * b);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 s = *reinterpret_cast<const float4*>(f + 16 * c + 4 * j);
+                    fma_pair(acc[8 * c + 2 * j], as_pair(r[c & 1][4 * j], r[c & 1][4 * j + 1]), make_float2(s.x, s.y));
+                    fma_pair(acc[8 * c + 2 * j + 1], as_pair(r[c & 1][4 * j + 2], r[c & 1][4 * j + 3]), make_float2(s.z, s.w));
+                }
+            }
+        }
+        if (!ok && lane == 0 && p.status != nullptr) *p.status = MM_TIMEOUT;
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 5) tmem_free(tmem, C::TMEM);
+    if (S > 1) {
+        float* sums = reinterpret_cast<float*>(smem);  // [T][128]
+        if (warp < 4) {
+#pragma unroll
+            for (int j = 0; j < T / 2; ++j) {
+                sums[(2 * j) * 128 + warp * 32 + lane] = acc[j].x;
+                sums[(2 * j + 1) * 128 + warp * 32 + lane] = acc[j].y;
+            }
+        }
+        cluster_sync();
+        if (warp < 4 && n < p.N) {
+            const float bias = load_bias(p, n);
+            for (int j = rank; j < T && m0 + j < p.M; j += S) {
+                float v = bias;
+                for (int q = 0; q < S; ++q) v += ld_cluster(base + (uint32_t)(j * 128 + warp * 32 + lane) * 4u, q);
+                static_cast<OUT*>(p.y)[(long long)(m0 + j) * p.y_stride + n] = from_f32<OUT>(v);
+            }
+        }
+        cluster_sync();
+    } else if (warp < 4 && n < p.N) {
+        const float bias = load_bias(p, n);
+        OUT* y = static_cast<OUT*>(p.y) + (long long)m0 * p.y_stride + n;
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+            if (m0 + j < p.M) y[j * p.y_stride] = from_f32<OUT>(bias + (j & 1 ? acc[j / 2].y : acc[j / 2].x));
+    }
 }
 
 }  // namespace qssm

@@ -41,7 +41,7 @@ __device__ __forceinline__ unsigned long long global_timer_ns() {
     return t;
 }
 // Bounded wait: gives up after about two seconds.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity) {
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity) {
     const unsigned long long t0 = global_timer_ns();
     for (uint32_t it = 0;; ++it) {
         if (mbar_try_wait(bar, parity)) return true;

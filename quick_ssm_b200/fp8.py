@@ -183,7 +183,10 @@ def matmul_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, *,
             rows *= n
         xv, xs = xv.reshape(rows, K), xs.reshape(rows, xs.shape[-1])
     y = torch.empty((xv.shape[0], N), dtype=out_dtype, device=xv.device)
-    _lib.matmul_fp8(_copyable(xv), xs, _copyable(wv), ws, bias, y)
+    if K == 0:  # an empty sum
+        y.copy_(bias) if bias is not None else y.zero_()
+    else:
+        _lib.matmul_fp8(_copyable(xv), xs, _copyable(wv), ws, bias, y)
     return y if len(lead) == 1 else y.view(*lead, N)
 
 

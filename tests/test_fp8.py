@@ -211,7 +211,8 @@ def check_product(y, x, w, bias, name=""):
 # both sides of every tile boundary, rows for one to many tokens, short and long sums, odd sizes
 PRODUCTS = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (2, 130, 100), (7, 1000, 257), (16, 256, 1024), (17, 129, 640),
             (33, 512, 4096), (64, 1024, 384), (65, 300, 1100), (127, 128, 128), (128, 256, 512), (129, 257, 129),
-            (200, 2500, 1100), (256, 256, 256), (257, 513, 130), (1000, 130, 48), (1537, 700, 260), (300, 8, 2000)]
+            (200, 2500, 1100), (256, 256, 256), (257, 513, 130), (1000, 130, 48), (1537, 700, 260), (300, 8, 2000),
+            (2100, 2500, 260), (129, 19001, 129), (9600, 514, 400), (4700, 1030, 16)]
 
 
 @gpu
