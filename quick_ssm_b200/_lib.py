@@ -442,84 +442,106 @@ def rmsnorm_bwd(x, w, dy, rstd, dx, dw) -> None:
     _rc(rc, "qssm_rmsnorm_bwd")
 
 
-def _pitch(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.stride(0)
+# The wrappers below serve single tokens too, where the host's time is the call's time: the device is compared by
+# ordinal, the current stream asked for as a plain handle, and each tensor's attributes are read once.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _ordinal(first: torch.Tensor, *others) -> int:
+    """Device ordinal that all tensors (None is skipped) share."""
+    index = first.get_device() if first.is_cuda else -1
+    if index < 0:
+        raise RuntimeError("the qssm kernels need CUDA tensors; there is no CPU path")
+    for t in others:
+        if t is not None and (not t.is_cuda or t.get_device() != index):
+            _require_cuda(first, *others)
+    return index
+
+
+def _call(fn, name: str, index: int, args) -> None:
+    """``fn(*args, stream)`` with device ``index`` current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc != 0:
+        _rc(rc, name)
 
 
 def add_rmsnorm_fwd(x, res, w, y, h, rstd, eps: float) -> None:
     """All but ``w`` and ``rstd`` are [rows, H] with a contiguous last axis; h = x + res, y = rms_norm(h) * w."""
-    dev = _require_cuda(x, res, w, y, h, rstd)
+    index = _ordinal(x, res, w)
+    lib = _lib or load()
     rows, H = x.shape
-    if _lib is None:
-        load()
-    with _on_device(dev):
-        rc = _lib.qssm_add_rmsnorm_fwd(_ptr(x), _ptr(res), _ptr(w), _ptr(y), _ptr(h), _ptr(rstd), rows, H, x.stride(0),
-                                       res.stride(0), y.stride(0), h.stride(0), eps, dtype_code(x.dtype),
-                                       dtype_code(res.dtype), dtype_code(w.dtype), _stream(dev))
-    if rc != 0:
-        _rc(rc, "qssm_add_rmsnorm_fwd")
+    _call(lib.qssm_add_rmsnorm_fwd, "qssm_add_rmsnorm_fwd", index,
+          (x.data_ptr(), res.data_ptr(), w.data_ptr(), y.data_ptr(), h.data_ptr(), None if rstd is None else rstd.data_ptr(),
+           rows, H, x.stride(0), res.stride(0), y.stride(0), h.stride(0), eps, _DTYPE_CODE[x.dtype],
+           _DTYPE_CODE[res.dtype], _DTYPE_CODE[w.dtype]))
 
 
 def add_rmsnorm_fp8(x, res, w, q, scales, h, eps: float) -> None:
     """As ``add_rmsnorm_fwd`` with y left in e4m3 ``q`` [rows, H] and ``scales`` [rows, blocks]; res and h may be None."""
-    dev = _require_cuda(x, res, w, q, scales, h)
+    index = _ordinal(x, res, w)
+    lib = _lib or load()
     rows, H = x.shape
-    if _lib is None:
-        load()
-    with _on_device(dev):
-        code = dtype_code(x.dtype)
-        rc = _lib.qssm_add_rmsnorm_fp8(_ptr(x), _ptr(res), _ptr(w), _ptr(q), _ptr(scales), _ptr(h), rows, H, x.stride(0),
-                                       _pitch(res), q.stride(0), _pitch(h), scales.stride(0), scales.stride(1), eps,
-                                       code, code if res is None else dtype_code(res.dtype), dtype_code(w.dtype),
-                                       _stream(dev))
-    if rc != 0:
-        _rc(rc, "qssm_add_rmsnorm_fp8")
+    code = _DTYPE_CODE[x.dtype]
+    srow, sblk = scales.stride()
+    if res is None:
+        rp, hp, rs, hs, rcode = None, None, 0, 0, code
+    else:
+        rp, hp, rs, hs, rcode = res.data_ptr(), h.data_ptr(), res.stride(0), h.stride(0), _DTYPE_CODE[res.dtype]
+    _call(lib.qssm_add_rmsnorm_fp8, "qssm_add_rmsnorm_fp8", index,
+          (x.data_ptr(), rp, w.data_ptr(), q.data_ptr(), scales.data_ptr(), hp, rows, H, x.stride(0), rs, q.stride(0), hs,
+           srow, sblk, eps, code, rcode, _DTYPE_CODE[w.dtype]))
 
 
 def add_rmsnorm_bwd(h, w, dy, dh, rstd, dx, dres, dw) -> None:
     """Gradients of ``add_rmsnorm_fwd``; dh, dx, dres may be None (not both of the last two)."""
-    dev = _require_cuda(h, w, dy, dh, rstd, dx, dres, dw)
+    index = _ordinal(h, dy, dh)
+    lib = _lib or load()
     rows, H = h.shape
-    if _lib is None:
-        load()
-    with _on_device(dev):
-        nbytes = int(_lib.qssm_add_rmsnorm_workspace_bytes(rows, H))
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        rc = _lib.qssm_add_rmsnorm_bwd(_ptr(h), _ptr(w), _ptr(dy), _ptr(dh), _ptr(rstd), _ptr(dx), _ptr(dres), _ptr(dw),
-                                       _ptr(ws), nbytes, rows, H, h.stride(0), dy.stride(0), _pitch(dh), _pitch(dx),
-                                       _pitch(dres), dtype_code(dy.dtype), dtype_code(h.dtype), dtype_code(w.dtype),
-                                       _stream(dev))
-    if rc != 0:
-        _rc(rc, "qssm_add_rmsnorm_bwd")
+    with _on_device(h.device):
+        nbytes = int(lib.qssm_add_rmsnorm_workspace_bytes(rows, H))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
+
+    def at(t):
+        return (None, 0) if t is None else (t.data_ptr(), t.stride(0))
+
+    (ep, es), (xp, xs), (rp, rs) = at(dh), at(dx), at(dres)
+    _call(lib.qssm_add_rmsnorm_bwd, "qssm_add_rmsnorm_bwd", index,
+          (h.data_ptr(), w.data_ptr(), dy.data_ptr(), ep, rstd.data_ptr(), xp, rp, dw.data_ptr(), ws.data_ptr(), nbytes,
+           rows, H, h.stride(0), dy.stride(0), es, xs, rs, _DTYPE_CODE[dy.dtype], _DTYPE_CODE[h.dtype],
+           _DTYPE_CODE[w.dtype]))
 
 
 def quant_fp8(x, q, scales, blocks: bool) -> None:
     """e4m3 values ``q`` and ``scales`` of [rows, K] ``x``: per 128 of a row, or (``blocks``) per 128 x 128."""
-    dev = _require_cuda(x, q, scales)
+    index = _ordinal(x)
+    lib = _lib or load()
     rows, K = x.shape
-    if _lib is None:
-        load()
-    with _on_device(dev):
-        fn = _lib.qssm_quant_fp8_blocks if blocks else _lib.qssm_quant_fp8_rows
-        rc = fn(_ptr(x), _ptr(q), _ptr(scales), rows, K, x.stride(0), q.stride(0), scales.stride(0), scales.stride(1),
-                dtype_code(x.dtype), _stream(dev))
-    if rc != 0:
-        _rc(rc, "qssm_quant_fp8")
+    srow, sblk = scales.stride()
+    _call(lib.qssm_quant_fp8_blocks if blocks else lib.qssm_quant_fp8_rows, "qssm_quant_fp8", index,
+          (x.data_ptr(), q.data_ptr(), scales.data_ptr(), rows, K, x.stride(0), q.stride(0), srow, sblk,
+           _DTYPE_CODE[x.dtype]))
 
 
 def matmul_fp8(x, x_scales, w, w_scales, bias, y) -> None:
     """y [M, N] = x [M, K] @ w [N, K]^T + bias on e4m3 operands whose rows start on 16-byte boundaries."""
-    dev = _require_cuda(x, x_scales, w, w_scales, bias, y)
+    index = _ordinal(x, x_scales, w, w_scales, bias)
+    if _lib is None:
+        load()
+    e = _status_words.get(index) or _status_entry(index)
+    if e[2].value != 0:
+        _raise_status(e)
     M, K = x.shape
-    status = _begin(dev)
-    with _on_device(dev):
-        rc = _lib.qssm_matmul_fp8(x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), _ptr(bias),
-                                  y.data_ptr(), M, w.shape[0], K, x.stride(0), x_scales.stride(0), x_scales.stride(1),
-                                  w.stride(0), w_scales.stride(0), w_scales.stride(1), y.stride(0),
-                                  dtype_code(y.dtype), 0 if bias is None else dtype_code(bias.dtype), status,
-                                  _stream(dev))
-    if rc != 0:
-        _rc(rc, "qssm_matmul_fp8")
+    xr, xb = x_scales.stride()
+    wr, wb = w_scales.stride()
+    bp, bcode = (None, 0) if bias is None else (bias.data_ptr(), _DTYPE_CODE[bias.dtype])
+    _call(_lib.qssm_matmul_fp8, "qssm_matmul_fp8", index,
+          (x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), bp, y.data_ptr(), M, w.shape[0], K,
+           x.stride(0), xr, xb, w.stride(0), wr, wb, y.stride(0), _DTYPE_CODE[y.dtype], bcode, e[1]))
 
 
 MAX_PEERS, PEER_SLOTS = 16, 4

@@ -30,21 +30,23 @@ int quant_check(const void* x, const void* q, const void* scales, long long rows
     return 0;
 }
 
-// e4m3 [rows, K] as the product's copies see it: boxes of 128 bytes of k and `box_rows` rows in the 128-byte swizzle,
-// zeros outside.  Each host thread keeps the maps it encoded last, as the scan does.
-int fp8_map(CUtensorMap& map, const void* ptr, long long rows, long long K, long long stride, int box_rows) {
+// [rows, cols] as the product's copies see it: boxes of 128 bytes x `box_rows` rows in the 128-byte swizzle, zeros
+// outside.  Each host thread keeps the maps it encoded last, as the scan does.  dtype: QSSM_* or -1 for bytes.
+int matrix_map(CUtensorMap& map, const void* ptr, long long rows, long long cols, long long pitch_bytes, int dtype, int box_rows) {
     struct Key {
         const void* ptr;
-        long long rows, K, stride, box;
+        long long rows, cols, pitch;
+        int dtype, box;
         bool operator==(const Key& o) const {
-            return ptr == o.ptr && rows == o.rows && K == o.K && stride == o.stride && box == o.box;
+            return ptr == o.ptr && rows == o.rows && cols == o.cols && pitch == o.pitch && dtype == o.dtype && box == o.box;
         }
     };
     struct Entry { Key key; CUtensorMap map; };
     static thread_local Entry cache[64];
     static thread_local bool have_context = false;
-    const Key key{ptr, rows, K, stride, box_rows};
-    const unsigned long long hash = ((unsigned long long)reinterpret_cast<uintptr_t>(ptr) + 64ull * box_rows + rows) * 0x9E3779B97F4A7C15ull;
+    const Key key{ptr, rows, cols, pitch_bytes, dtype, box_rows};
+    const unsigned long long hash =
+        ((unsigned long long)reinterpret_cast<uintptr_t>(ptr) + 64ull * box_rows + rows + dtype) * 0x9E3779B97F4A7C15ull;
     Entry& e = cache[hash >> 58];
     if (e.key == key) {
         map = e.map;
@@ -56,11 +58,14 @@ int fp8_map(CUtensorMap& map, const void* ptr, long long rows, long long K, long
     }
     EncodeTiledFn enc = encode_fn();
     if (enc == nullptr) return QSSM_E_DRIVER;
-    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
-    cuuint32_t box[2] = {(cuuint32_t)MM_TILE_K, (cuuint32_t)box_rows}, estr[2] = {1u, 1u};
-    if (enc(&e.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    const CUtensorMapDataType type = dtype == QSSM_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : dtype == QSSM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                     : dtype == QSSM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const int es = dtype < 0 ? 1 : dtype_size(dtype);
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch_bytes};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows}, estr[2] = {1u, 1u};
+    if (enc(&e.map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
         e.key.ptr = nullptr;
         return QSSM_E_STRIDE;
     }
@@ -78,7 +83,7 @@ struct MatmulPlan {
 MatmulPlan plan_matmul(long long M, long long N, int n_kb) {
     const long long sms = sm_count();
     const long long big = ((M + MMR_M - 1) / MMR_M) * ((N + MMR_N - 1) / MMR_N);
-    if (M > 64 && big >= sms) return {0, 1, MMR_M, MMR_N};
+    if (M > 64 && big >= sms / 2) return {0, 1, 128, 128};
     const int T = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const long long tiles = ((N + 127) / 128) * ((M + T - 1) / T);
     int S = 1;
@@ -169,8 +174,10 @@ int qssm_matmul_fp8(const void* x, const float* x_scales, const void* w, const f
     p.y_vec = fits(y, y_stride, 16, es);
     const MatmulPlan plan = plan_matmul(M, N, p.n_kb);
     int rc;
-    if ((rc = fp8_map(p.x_map, x, M, K, x_stride, plan.x_box)) || (rc = fp8_map(p.w_map, w, N, K, w_stride, plan.w_box)))
+    if ((rc = matrix_map(p.x_map, x, M, K, x_stride, -1, plan.x_box)) ||
+        (rc = matrix_map(p.w_map, w, N, K, w_stride, -1, plan.w_box)))
         return rc;
+    if (plan.T == 0 && p.y_vec && (rc = matrix_map(p.y_map, y, M, N, y_stride * es, out_dtype, 32))) return rc;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     return with_type(out_dtype, [&](auto t) -> int {
         using T = decltype(t);
@@ -180,7 +187,8 @@ int qssm_matmul_fp8(const void* x, const float* x_scales, const void* w, const f
             const long long tiles = (long long)p.m_tiles * p.n_tiles;
             if (tiles >= (1ll << 31) - 1024) return QSSM_E_SHAPE;
             if ((rc = ensure_smem(matmul_fp8_rows_kernel<T>, MMR_SMEM))) return rc;
-            const unsigned grid = (unsigned)(tiles < sm_count() ? tiles : sm_count());
+            const int pairs = sm_count() / 2;
+            const unsigned grid = 2u * (unsigned)(tiles < pairs ? tiles : pairs);
             matmul_fp8_rows_kernel<T><<<grid, MMR_THREADS, MMR_SMEM, stream>>>(p);
             return (int)cudaGetLastError();
         }

@@ -17,7 +17,7 @@
 namespace qssm {
 
 struct MatmulParams {
-    CUtensorMap x_map, w_map;
+    CUtensorMap x_map, w_map, y_map;
     const float* x_scales;  // [M, K/128]
     const float* w_scales;  // [N/128, K/128]
     const void* bias;       // [N] or NULL
@@ -41,87 +41,145 @@ __device__ __forceinline__ float load_bias(const MatmulParams& p, int n) {
 __device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows: tiles of 128 rows x 256 columns, a persistent CTA per SM.  Lane = row: a thread owns one row's sums of
-// 128 columns, and both scales of a block are one factor for all of them.
+// Many rows: two CTAs on neighbouring SMs form 256 x 256 tiles as one product (cta_group::2), each with 128 rows of x,
+// half of the weight's 256 rows in shared memory, and the sums of its 128 rows.  Against tiles of 128 x 256 by single
+// CTAs that is a third less to read from L2 per product.  Persistent: one pair per two SMs walks the tiles.
+//
+// Lane = row: a thread owns one row's sums of 128 columns, and both scales of a block are one factor for all of them.
+// A warp of its own fetches the factors ahead of their use.  Results leave through shared memory and bulk stores of
+// 32 rows x 128 bytes per warp, so that the sums' registers are free for the next tile at once.
 // ---------------------------------------------------------------------------------------------
-constexpr int MMR_M = 128, MMR_N = 256, MMR_STAGES = 4;
-constexpr int MMR_A = MMR_M * MM_TILE_K, MMR_STAGE = MMR_A + MMR_N * MM_TILE_K;
-constexpr int MMR_THREADS = 320;  // warps 0-7 sums, 8 copies, 9 products
-constexpr int MMR_SMEM = MMR_STAGES * MMR_STAGE + 8 * 128 * 4 + 256 + 1024;
+constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;  // a pair's tile
+constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
+constexpr int MMR_THREADS = 384;  // warps 0-7 sums, 8 copies, 9 products, 10 factors
+constexpr int MMR_FACTORS = 8;    // blocks of factors in flight
+constexpr int MMR_OUT = MMR_STAGES * MMR_STAGE, MMR_BIAS = MMR_OUT + 8 * 2 * 4096, MMR_FACT = MMR_BIAS + 8 * 512,
+              MMR_BARS = MMR_FACT + MMR_FACTORS * 1024, MMR_SMEM = MMR_BARS + 256 + 1024;
+// Registers: 168 a thread at launch (384 threads); the four helper warps give 96 of theirs to the eight others.
+constexpr int MMR_REGS_SUMS = 216, MMR_REGS_HELP = 72;
+static_assert(256 * MMR_REGS_SUMS + 128 * MMR_REGS_HELP <= 384 * 168, "more registers than the CTA has");
 
-template <typename T> __global__ void __launch_bounds__(MMR_THREADS, 1) matmul_fp8_rows_kernel(const __grid_constant__ MatmulParams p) {
+template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMR_THREADS, 1)
+    matmul_fp8_rows_kernel(const __grid_constant__ MatmulParams p) {
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    const uint32_t base = smem_u32(smem);
-    float* bias_at = reinterpret_cast<float*>(smem + MMR_STAGES * MMR_STAGE);
-    const uint32_t bars = base + MMR_STAGES * MMR_STAGE + 8 * 128 * 4;
-    const uint32_t full = bars, empty = full + 8 * MMR_STAGES, done = empty + 8 * MMR_STAGES, taken = done + 16, last = taken + 16;
+    const uint32_t base = smem_u32(smem), bars = base + MMR_BARS;
+    // full, taken: the even CTA's count for both; the others are each CTA's own
+    const uint32_t full = bars, empty = full + 8 * MMR_STAGES, done = empty + 8 * MMR_STAGES, taken = done + 16,
+                   fready = taken + 16, fused = fready + 8 * MMR_FACTORS, last = fused + 8 * MMR_FACTORS;
+    static_assert(8 * (2 * MMR_STAGES + 4 + 2 * MMR_FACTORS + 1) + 4 <= 256, "room for the barriers");
     volatile uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + (last + 8 - base));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
     if (threadIdx.x == 0) {
         for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, 8); }
+        for (int b = 0; b < 2; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, 16); }
+        for (int f = 0; f < MMR_FACTORS; ++f) { mbar_init(fready + 8 * f, 1); mbar_init(fused + 8 * f, 8); }
         mbar_init(last, 1);
         fence_barrier_init();
     }
-    if (warp == 9) tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_at)), 512);
+    if (warp == 9) tmem_alloc<2>(smem_u32(const_cast<uint32_t*>(tmem_at)), 512);
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
-    const int tiles = p.m_tiles * p.n_tiles;
+    const int tiles = p.m_tiles * p.n_tiles, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    bool ok = true;
 
-    if (warp == 8) {
-        if (lane == 0) {
+    if (warp >= 8) {
+        regs_down<MMR_REGS_HELP>();
+        if (warp == 8 && lane == 0) {
             prefetch_map(&p.x_map);
             prefetch_map(&p.w_map);
+            const uint32_t full0 = cluster_addr(full, 0);
             uint32_t it = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                const int m0 = (t % p.m_tiles) * MMR_M, n0 = (t / p.m_tiles) * MMR_N;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N + (int)rank * 128;
                 for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
                     const uint32_t s = it % MMR_STAGES, round = it / MMR_STAGES;
                     if (round > 0 && !mbar_wait_limit(empty + 8 * s, (round - 1) & 1)) { ok = false; break; }
-                    mbar_expect_tx(full + 8 * s, MMR_STAGE);
-                    tma_load_2d(base + s * MMR_STAGE, &p.x_map, full + 8 * s, kb * MM_TILE_K, m0);
-                    tma_load_2d(base + s * MMR_STAGE + MMR_A, &p.w_map, full + 8 * s, kb * MM_TILE_K, n0);
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * MMR_STAGE);
+                    tma_load_2d_pair(base + s * MMR_STAGE, &p.x_map, full0 + 8 * s, kb * MM_TILE_K, m0);
+                    tma_load_2d_pair(base + s * MMR_STAGE + MMR_A, &p.w_map, full0 + 8 * s, kb * MM_TILE_K, n0);
                 }
             }
-            // no copy outlives the CTA
+            // no copy outlives the pair: the last rounds' products are done (both CTAs are told), or time is given
             const uint32_t left = it < (uint32_t)MMR_STAGES ? it : (uint32_t)MMR_STAGES;
-            for (uint32_t i = it - left; i < it; ++i) ok &= mbar_wait_limit(full + 8 * (i % MMR_STAGES), (i / MMR_STAGES) & 1);
-            if (!ok && p.status != nullptr) *p.status = MM_TIMEOUT;
-        }
-    } else if (warp == 9) {
-        if (lane == 0) {
+            for (uint32_t i = it - left; ok && i < it; ++i) ok = mbar_wait_limit(empty + 8 * (i % MMR_STAGES), (i / MMR_STAGES) & 1);
+            if (!ok) wait_ns(1000000);
+        } else if (warp == 9 && lane == 0 && rank == 0) {
             constexpr uint32_t idesc = fp8_idesc(MMR_M, MMR_N);
             uint32_t it = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            for (int t = pair; ok && t < tiles; t += pairs) {
                 for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
                     const uint32_t s = it % MMR_STAGES, b = it & 1;
                     if (it >= 2 && !mbar_wait_limit(taken + 8 * b, ((it >> 1) - 1) & 1)) { ok = false; break; }
                     if (!mbar_wait_limit(full + 8 * s, (it / MMR_STAGES) & 1)) { ok = false; break; }
                     tc_fence_after();
-                    const uint64_t a = smem_operand(base + s * MMR_STAGE), w = smem_operand(base + s * MMR_STAGE + MMR_A);
+                    const uint64_t x = smem_operand(base + s * MMR_STAGE), w = smem_operand(base + s * MMR_STAGE + MMR_A);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc_mma_fp8(tmem + b * MMR_N, a + 2 * k, w + 2 * k, idesc, k > 0);
-                    tc_commit(empty + 8 * s);
-                    tc_commit(done + 8 * b);
+                    for (int k = 0; k < 4; ++k) tc_mma_fp8_pair(tmem + b * MMR_N, x + 2 * k, w + 2 * k, idesc, k > 0);
+                    tc_commit_pair(empty + 8 * s);
+                    tc_commit_pair(done + 8 * b);
                 }
             }
-            tc_commit(last);  // no product outlives the CTA
+            tc_commit_group2(last);  // no product outlives the pair
             ok &= mbar_wait_limit(last, 0);
-            if (!ok && p.status != nullptr) *p.status = MM_TIMEOUT;
+        } else if (warp == 10) {
+            // factors of block kb: scale of the row x scale of the weight's block, for 128 rows x two halves of columns
+            float* out = reinterpret_cast<float*>(smem + MMR_FACT);
+            uint32_t it = 0;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N;
+                const float* xs[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int m = m0 + 32 * i + lane;
+                    xs[i] = p.x_scales + (long long)(m < p.M ? m : 0) * p.xs_row;
+                }
+                const float* w0 = p.w_scales + (long long)(n0 / 128) * p.ws_row;
+                const float* w1 = n0 + 128 < p.N ? w0 + p.ws_row : w0;
+                constexpr int AHEAD = 2;  // blocks fetched together
+                for (int kb0 = 0; ok && kb0 < p.n_kb; kb0 += AHEAD) {
+                    float x[AHEAD][4], w[AHEAD][2];
+#pragma unroll
+                    for (int a = 0; a < AHEAD; ++a) {
+                        const long long kb = kb0 + a < p.n_kb ? kb0 + a : kb0;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[a][i] = xs[i][kb * p.xs_blk];
+                        w[a][0] = w0[kb * p.ws_blk];
+                        w[a][1] = w1[kb * p.ws_blk];
+                    }
+#pragma unroll
+                    for (int a = 0; a < AHEAD; ++a) {
+                        if (kb0 + a >= p.n_kb) break;
+                        const uint32_t f = it % MMR_FACTORS, round = it / MMR_FACTORS;
+                        if (round > 0 && !mbar_wait_limit(fused + 8 * f, (round - 1) & 1)) { ok = false; break; }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            out[f * 256 + 32 * i + lane] = x[a][i] * w[a][0];
+                            out[f * 256 + 128 + 32 * i + lane] = x[a][i] * w[a][1];
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(fready + 8 * f);
+                        ++it;
+                    }
+                }
+            }
         }
     } else {
-        const int half = warp >> 2;
-        const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 128;
-        float* my_bias = bias_at + warp * 128;
+        regs_up<MMR_REGS_SUMS>();
+        const int half = warp >> 2, quarter = warp & 3;
+        const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
+        const uint32_t taken0 = cluster_addr(taken, 0);
+        float* my_bias = reinterpret_cast<float*>(smem + MMR_BIAS) + warp * 128;
+        const float* my_factor = reinterpret_cast<const float*>(smem + MMR_FACT) + half * 128 + quarter * 32 + lane;
+        const uint32_t out = base + MMR_OUT + warp * 8192;
+        uint8_t* const out_row = smem + MMR_OUT + warp * 8192 + lane * 128;
         uint32_t it = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-            const int m = (t % p.m_tiles) * MMR_M + (warp & 3) * 32 + lane, n0 = (t / p.m_tiles) * MMR_N + half * 128;
+        for (int t = pair; ok && t < tiles; t += pairs) {
+            const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + quarter * 32, n0 = (t / p.m_tiles) * MMR_N + half * 128;
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < 4; ++i) my_bias[i * 32 + lane] = load_bias(p, n0 + i * 32 + lane);
@@ -133,17 +191,15 @@ template <typename T> __global__ void __launch_bounds__(MMR_THREADS, 1) matmul_f
                 acc[2 * j] = make_float2(v.x, v.y);
                 acc[2 * j + 1] = make_float2(v.z, v.w);
             }
-            const float* xs = p.x_scales + (long long)(m < p.M ? m : 0) * p.xs_row;
-            const float* ws = p.w_scales + (long long)(n0 < p.N ? n0 / 128 : 0) * p.ws_row;
-            // scales two blocks ahead of their use
-            float s0 = xs[0] * ws[0], s1 = p.n_kb > 1 ? xs[p.xs_blk] * ws[p.ws_blk] : 0.f;
             for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
-                float xa = 0.f, wa = 0.f;
-                if (kb + 2 < p.n_kb) { xa = xs[(kb + 2) * p.xs_blk]; wa = ws[(kb + 2) * p.ws_blk]; }
-                const uint32_t b = it & 1;
+                const uint32_t b = it & 1, f = it % MMR_FACTORS;
+                if (!mbar_wait_limit(fready + 8 * f, (it / MMR_FACTORS) & 1)) { ok = false; break; }
+                const float factor = my_factor[f * 256];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(fused + 8 * f);
                 if (!mbar_wait_limit(done + 8 * b, (it >> 1) & 1)) { ok = false; break; }
                 tc_fence_after();
-                const float2 s = make_float2(s0, s0);
+                const float2 s = make_float2(factor, factor);
                 uint32_t r[2][32];
                 tmem_ld<32>(at + b * MMR_N, r[0]);
 #pragma unroll
@@ -152,39 +208,61 @@ template <typename T> __global__ void __launch_bounds__(MMR_THREADS, 1) matmul_f
                     if (c < 3) tmem_ld<32>(at + b * MMR_N + 32 * (c + 1), r[(c + 1) & 1]);
                     else {  // all read: the buffer may be written again
                         tc_fence_before();
-                        if (lane == 0) mbar_arrive(taken + 8 * b);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(taken0 + 8 * b);
                     }
 #pragma unroll
                     for (int j = 0; j < 16; ++j) fma_pair(acc[16 * c + j], as_pair(r[c & 1][2 * j], r[c & 1][2 * j + 1]), s);
                 }
-                s0 = s1;
-                s1 = xa * wa;
             }
-            if (!ok) break;
-            if (m < p.M) {
-                T* yr = static_cast<T*>(p.y) + (long long)m * p.y_stride + n0;
-                constexpr int V = 16 / sizeof(T);
+            if (!ok || m0 >= p.M || n0 >= p.N) continue;
+            // 128 bytes of each row at a time; 16-byte piece c of row r lies at c ^ (r & 7), where a bulk store in the
+            // 128-byte swizzle looks for it, and eight lanes' pieces in eight different banks
+            constexpr int V = 16 / sizeof(T), COLS = 8 * V, CHUNKS = 128 / COLS;
 #pragma unroll
-                for (int j = 0; j < 128; j += V) {
+            for (int c = 0; c < CHUNKS; ++c) {
+                if (lane == 0) tma_wait_read<1>();  // the store that read this buffer before
+                __syncwarp();
+                uint8_t* row = out_row + (c & 1) * 4096;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
                     float v[V];
 #pragma unroll
-                    for (int i = 0; i < V; i += 2) { v[i] = acc[(j + i) / 2].x; v[i + 1] = acc[(j + i) / 2].y; }
-                    if (p.y_vec && n0 + j + V <= p.N) store_elems<T, V>(yr + j, v);
-                    else {
+                    for (int i = 0; i < V; i += 2) {
+                        v[i] = acc[(c * COLS + q * V + i) / 2].x;
+                        v[i + 1] = acc[(c * COLS + q * V + i) / 2].y;
+                    }
+                    store_elems<T, V>(reinterpret_cast<T*>(row + ((q ^ (lane & 7)) << 4)), v);
+                }
+                if (p.y_vec) {
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (n0 + c * COLS < p.N) tma_store_2d(&p.y_map, out + (c & 1) * 4096, n0 + c * COLS, m0);
+                        tma_commit();
+                    }
+                } else {  // rows of y on any boundary: each row's piece by consecutive lanes
+                    __syncwarp();
+                    const int rows = p.M - m0 < 32 ? p.M - m0 : 32, cols = p.N - n0 - c * COLS;
+                    for (int r = 0; r < rows; ++r) {
+                        const uint8_t* src = smem + MMR_OUT + warp * 8192 + (c & 1) * 4096 + r * 128;
+                        T* dst = static_cast<T*>(p.y) + (long long)(m0 + r) * p.y_stride + n0 + c * COLS;
 #pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            if (n0 + j + i < p.N) yr[j + i] = from_f32<T>(v[i]);
+                        for (int i = lane; i < COLS; i += 32)
+                            if (i < cols) dst[i] = *reinterpret_cast<const T*>(src + (((i / V) ^ (r & 7)) << 4) + (i % V) * sizeof(T));
                     }
                 }
             }
         }
-        if (!ok && lane == 0 && p.status != nullptr) *p.status = MM_TIMEOUT;
+        if (lane == 0) tma_wait_all();
     }
+    if (!ok && lane == 0 && p.status != nullptr) *p.status = MM_TIMEOUT;
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     tc_fence_after();
-    if (warp == 9) tmem_free(tmem, 512);
+    if (warp == 9) tmem_free<2>(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -219,7 +297,7 @@ template <typename OUT, int T> __global__ void __launch_bounds__(MMF_THREADS, 2)
         mbar_init(last, 1);
         fence_barrier_init();
     }
-    if (warp == 5) tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_at)), C::TMEM);
+    if (warp == 5) tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_at)), C::TMEM);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -326,7 +404,7 @@ template <typename OUT, int T> __global__ void __launch_bounds__(MMF_THREADS, 2)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 5) tmem_free(tmem, C::TMEM);
+    if (warp == 5) tmem_free<1>(tmem, C::TMEM);
     if (S > 1) {
         float* sums = reinterpret_cast<float*>(smem);  // [T][128]
         if (warp < 4) {

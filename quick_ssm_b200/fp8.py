@@ -17,7 +17,7 @@ from . import _lib
 
 BLOCK = 128
 _E4M3 = torch.float8_e4m3fn
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
 
 
 def n_blocks(size: int) -> int:
@@ -31,7 +31,7 @@ def rows_2d(t: torch.Tensor) -> torch.Tensor:
         for n in t.shape[:-1]:
             rows *= n
         t = t.reshape(rows, t.shape[-1])
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
 class Fp8Rows:
@@ -40,14 +40,19 @@ class Fp8Rows:
     __slots__ = ("values", "scales")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
-        if values.dtype != _E4M3 or scales.dtype != torch.float32:
+        if values.dtype is not _E4M3 or scales.dtype is not torch.float32:
             raise TypeError(f"values must be float8_e4m3fn and scales float32; got {values.dtype} and {scales.dtype}")
-        if values.dim() < 1 or scales.shape[:-1] != values.shape[:-1] or scales.dim() != values.dim() \
-                or scales.shape[-1] != n_blocks(values.shape[-1]):
+        *lead, K = values.shape
+        if [*lead, n_blocks(K)] != list(scales.shape):
             raise ValueError(f"scales {tuple(scales.shape)} are not one for each 128 of a row of {tuple(values.shape)}")
-        if scales.device != values.device:
-            raise RuntimeError("values and scales must live on the same device")
         self.values, self.scales = values, scales
+
+    @classmethod
+    def _of(cls, values: torch.Tensor, scales: torch.Tensor) -> "Fp8Rows":
+        """What this package has made itself: nothing to check."""
+        q = cls.__new__(cls)
+        q.values, q.scales = values, scales
+        return q
 
     @property
     def shape(self) -> torch.Size:
@@ -57,12 +62,14 @@ class Fp8Rows:
     def device(self) -> torch.device:
         return self.values.device
 
-    def view_as_rows_of(self, shape) -> "Fp8Rows":
-        """The same rows under leading axes ``shape[:-1]``."""
+    def _under(self, shape) -> "Fp8Rows":
+        """[rows, K] as the same rows under leading axes ``shape[:-1]``."""
         if len(shape) == 2:
             return self
-        return Fp8Rows(self.values.unflatten(0, tuple(shape[:-1])) if len(shape) > 2 else self.values[0],
-                       self.scales.unflatten(0, tuple(shape[:-1])) if len(shape) > 2 else self.scales[0])
+        if len(shape) == 1:
+            return Fp8Rows._of(self.values[0], self.scales[0])
+        lead = tuple(shape[:-1])
+        return Fp8Rows._of(self.values.unflatten(0, lead), self.scales.unflatten(0, lead))
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         per = self.scales.repeat_interleave(BLOCK, -1)[..., :self.values.shape[-1]]
@@ -75,13 +82,10 @@ class Fp8Weight:
     __slots__ = ("values", "scales")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
-        if values.dtype != _E4M3 or scales.dtype != torch.float32:
+        if values.dtype is not _E4M3 or scales.dtype is not torch.float32:
             raise TypeError(f"values must be float8_e4m3fn and scales float32; got {values.dtype} and {scales.dtype}")
-        if values.dim() != 2 or scales.dim() != 2 or scales.shape[0] != n_blocks(values.shape[0]) \
-                or scales.shape[1] != n_blocks(values.shape[1]):
+        if values.dim() != 2 or [n_blocks(n) for n in values.shape] != list(scales.shape):
             raise ValueError(f"scales {tuple(scales.shape)} are not one for each 128 x 128 block of {tuple(values.shape)}")
-        if scales.device != values.device:
-            raise RuntimeError("values and scales must live on the same device")
         self.values, self.scales = values, scales
 
     @property
@@ -100,27 +104,24 @@ class Fp8Weight:
 
 def _values_like(rows: int, K: int, device) -> torch.Tensor:
     """e4m3 [rows, K] whose rows start on 16-byte boundaries, as the product's copies need them."""
-    pitch = (K + 15) // 16 * 16
-    q = torch.empty((rows, pitch), dtype=_E4M3, device=device)
-    return q if pitch == K else q[:, :K]
+    return torch.empty_strided((rows, K), ((K + 15) // 16 * 16, 1), dtype=_E4M3, device=device)
 
 
 def rows_like(x2: torch.Tensor) -> Fp8Rows:
     """Room for the quantised rows of [rows, K] ``x2``.  The scales lie block by block (all rows of a block side by
     side): 32 rows of a product's tile then read theirs in one access."""
     rows, K = x2.shape
-    return Fp8Rows(_values_like(rows, K, x2.device),
-                   torch.empty((n_blocks(K), rows), dtype=torch.float32, device=x2.device).t())
+    dev = x2.device
+    return Fp8Rows._of(_values_like(rows, K, dev), torch.empty_strided((rows, n_blocks(K)), (1, rows), dtype=torch.float32, device=dev))
 
 
 def _check_source(x: torch.Tensor, name: str) -> None:
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise RuntimeError(f"{name} needs CUDA tensors; there is no CPU path")
     if x.dtype not in _FLOATS:
         raise TypeError(f"{name} takes float32, float16 and bfloat16; got {x.dtype}")
 
 
-@torch.no_grad()
 def quantize_rows(x: torch.Tensor) -> Fp8Rows:
     """Quantise ``[..., K]`` activations, one scale for each 128 values of a row."""
     _check_source(x, "quantize_rows")
@@ -129,10 +130,9 @@ def quantize_rows(x: torch.Tensor) -> Fp8Rows:
     x2 = rows_2d(x)
     q = rows_like(x2)
     _lib.quant_fp8(x2, q.values, q.scales, False)
-    return q.view_as_rows_of(x.shape)
+    return q._under(x.shape)
 
 
-@torch.no_grad()
 def quantize_weight(w: torch.Tensor) -> Fp8Weight:
     """Quantise an ``[N, K]`` weight (``torch.nn.Linear`` layout), one scale for each 128 x 128 block."""
     _check_source(w, "quantize_weight")
@@ -150,20 +150,19 @@ def _copyable(values: torch.Tensor) -> torch.Tensor:
     """[rows, K] values as the product's copies can address them: a copy where a row or the base is not on a 16-byte
     boundary or the last axis is strided."""
     rows, K = values.shape
-    if (values.stride(1) == 1 or K <= 1) and values.data_ptr() % 16 == 0 and values.stride(0) % 16 == 0 \
-            and values.stride(0) >= K:
+    pitch, step = values.stride()
+    if (step == 1 or K <= 1) and pitch % 16 == 0 and pitch >= K and values.data_ptr() % 16 == 0:
         return values
     out = _values_like(rows, K, values.device)
     out.copy_(values)
     return out
 
 
-@torch.no_grad()
 def matmul_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, *,
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x @ w.T + bias`` on quantised operands: ``[..., N]`` in ``out_dtype`` (bf16, fp16 or fp32)."""
     xv, xs, wv, ws = x.values, x.scales, w.values, w.scales
-    if xv.device.type != "cuda":
+    if not xv.is_cuda:
         raise RuntimeError("matmul_fp8 needs CUDA tensors; there is no CPU path")
     if out_dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be float32, float16 or bfloat16; got {out_dtype}")
@@ -175,14 +174,14 @@ def matmul_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, *,
             raise ValueError(f"bias is {tuple(bias.shape)}, expected {(N,)}")
         if bias.dtype not in _FLOATS:
             raise TypeError(f"bias must be float32, float16 or bfloat16; got {bias.dtype}")
-        bias = bias.contiguous()
+        bias = bias.detach().contiguous()
     lead = xv.shape[:-1]
     if xv.dim() != 2:
         rows = 1
         for n in lead:
             rows *= n
         xv, xs = xv.reshape(rows, K), xs.reshape(rows, xs.shape[-1])
-    y = torch.empty((xv.shape[0], N), dtype=out_dtype, device=xv.device)
+    y = torch.empty_strided((xv.shape[0], N), (N, 1), dtype=out_dtype, device=xv.device)
     if K == 0:  # an empty sum
         y.copy_(bias) if bias is not None else y.zero_()
     else:

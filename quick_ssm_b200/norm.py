@@ -63,54 +63,63 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.
     return _RMSNormFunction.apply(x, weight, eps)
 
 
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
 
 
 def _check_add(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, name: str) -> None:
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise RuntimeError(f"{name} needs CUDA tensors; there is no CPU path")
-    if x.dtype not in _FLOATS or weight.dtype not in _FLOATS:
-        raise TypeError(f"{name} takes float32, float16 and bfloat16; got {x.dtype} with a weight in {weight.dtype}")
-    if x.dim() < 1 or weight.shape != x.shape[-1:]:
+    dt, shape = x.dtype, x.shape
+    if dt not in _FLOATS or weight.dtype not in _FLOATS:
+        raise TypeError(f"{name} takes float32, float16 and bfloat16; got {dt} with a weight in {weight.dtype}")
+    if len(shape) < 1 or weight.shape != shape[-1:]:
         raise ValueError("weight must have the size of the last axis of x")
     if residual is not None:
-        if residual.shape != x.shape:
-            raise ValueError(f"residual is {tuple(residual.shape)}, x is {tuple(x.shape)}")
-        if residual.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"residual must be in x's type or in float32; got {residual.dtype} with x in {x.dtype}")
+        if residual.shape != shape:
+            raise ValueError(f"residual is {tuple(residual.shape)}, x is {tuple(shape)}")
+        if residual.dtype is not dt and residual.dtype is not torch.float32:
+            raise TypeError(f"residual must be in x's type or in float32; got {residual.dtype} with x in {dt}")
+
+
+def _dense(shape, dtype, device) -> torch.Tensor:
+    """An uninitialised contiguous tensor (``empty_strided`` takes two thirds of ``empty``'s time on the host)."""
+    strides, step = [], 1
+    for n in reversed(shape):
+        strides.append(step)
+        step *= max(n, 1)
+    return torch.empty_strided(tuple(shape), strides[::-1], dtype=dtype, device=device)
 
 
 class _AddRMSNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
         x2, r2, w = rows_2d(x), rows_2d(residual), weight.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-        rstd = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
+        dev = x.device
+        y = _dense(x.shape, x.dtype, dev)
+        h = _dense(x.shape, residual.dtype, dev)
+        rstd = torch.empty(x2.shape[0], dtype=torch.float32, device=dev) if any(ctx.needs_input_grad) else None
         _lib.add_rmsnorm_fwd(x2, r2, w, rows_2d(y), rows_2d(h), rstd, eps)
-        ctx.save_for_backward(h, w, rstd)
-        ctx.set_materialize_grads(False)
-        ctx.x_dtype = x.dtype
+        if rstd is not None:
+            ctx.save_for_backward(h, w, rstd)
+            ctx.set_materialize_grads(False)
         return y, h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh):
+        if torch.is_grad_enabled():
+            raise RuntimeError("add_rms_norm has no second derivative")
         h, w, rstd = ctx.saved_tensors
         need_x, need_r, need_w, _ = ctx.needs_input_grad
-        shape, xd, rd = h.shape, ctx.x_dtype, h.dtype
-        h = rows_2d(h)
         if dy is None:  # only h was used: its gradient passes through
-            dx = dh.to(xd) if need_x and dh is not None else None
-            return dx, dh if need_r else None, None, None
-        dev = h.device
-        dx = torch.empty(h.shape, dtype=xd, device=dev) if need_x or rd == xd else None
-        dres = torch.empty(h.shape, dtype=rd, device=dev) if rd != xd and (need_r or dx is None) else None
-        dw = torch.empty(w.shape, dtype=w.dtype, device=dev)
-        _lib.add_rmsnorm_bwd(h, w, rows_2d(dy.to(xd)), None if dh is None else rows_2d(dh.to(rd)), rstd, dx, dres, dw)
-        gx = dx.view(shape) if need_x else None
-        gr = (dx if rd == xd else dres).view(shape) if need_r else None
-        return gx, gr, dw if need_w else None, None
+            return (dh if need_x else None), (dh if need_r else None), None, None
+        # autograd hands over gradients in the outputs' types and takes the inputs' own back
+        xd, rd, dev, shape = dy.dtype, h.dtype, h.device, h.shape
+        dx = _dense(shape, xd, dev) if need_x or rd is xd else None
+        dres = _dense(shape, rd, dev) if rd is not xd and (need_r or dx is None) else None
+        dw = _dense(w.shape, w.dtype, dev)
+        _lib.add_rmsnorm_bwd(rows_2d(h), w, rows_2d(dy), None if dh is None else rows_2d(dh), rstd,
+                             None if dx is None else rows_2d(dx), None if dres is None else rows_2d(dres), dw)
+        return (dx if need_x else None), ((dx if rd is xd else dres) if need_r else None), (dw if need_w else None), None
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
@@ -119,14 +128,13 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
 
     ``x``: ``[..., H]`` fp32, fp16 or bf16; ``residual``: the same shape, in x's type or in fp32 (a 32-bit residual
     stream under 16-bit branches).  ``y`` has x's type, ``h`` the residual's; the norm is that of ``h`` as stored.
-    Differentiable in x, residual and weight."""
-    _check_add(x, residual, weight, "add_rms_norm")
+    Differentiable (once) in x, residual and weight."""
     if residual is None:
         raise ValueError("add_rms_norm needs a residual; rms_norm is the norm alone")
+    _check_add(x, residual, weight, "add_rms_norm")
     return _AddRMSNormFunction.apply(x, residual, weight, float(eps))
 
 
-@torch.no_grad()
 def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
                      eps: float = 1e-5) -> Tuple[Fp8Rows, torch.Tensor]:
     """The sum and norm of ``add_rms_norm`` with y quantised for ``fp8.matmul_fp8``; returns ``(y, h)``.
@@ -135,8 +143,12 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
     stack): h is x itself.  Serving only, no gradient."""
     _check_add(x, residual, weight, "add_rms_norm_fp8")
     x2 = rows_2d(x)
-    r2 = None if residual is None else rows_2d(residual)
-    h = x if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
     q = rows_like(x2)
-    _lib.add_rmsnorm_fp8(x2, r2, weight.contiguous(), q.values, q.scales, None if residual is None else rows_2d(h), float(eps))
-    return q.view_as_rows_of(x.shape), h
+    w = weight.contiguous()
+    if residual is None:
+        h = x
+        _lib.add_rmsnorm_fp8(x2, None, w, q.values, q.scales, None, float(eps))
+    else:
+        h = _dense(x.shape, residual.dtype, x.device)
+        _lib.add_rmsnorm_fp8(x2, rows_2d(residual), w, q.values, q.scales, rows_2d(h), float(eps))
+    return q._under(x.shape), h
