@@ -5,13 +5,17 @@
 
 namespace qssm {
 
-// Waits until the barrier's phase `parity` has completed; gives up after about two seconds.
+// Waits until the barrier's phase `parity` has completed; gives up after about two seconds.  The timer is not read in
+// the first tries: reading it takes longer than most waits (about a microsecond).
 __device__ __forceinline__ bool mbar_wait_limit(uint32_t bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (int it = 0; it < 256; ++it)
+        if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long t0 = global_timer_ns();
+#pragma unroll 1
     for (uint32_t it = 0; it < (1u << 28); ++it) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63u) == 63u && global_timer_ns() - t0 > 2000000000ull) return false;
+        if ((it & 255u) == 255u && global_timer_ns() - t0 > 2000000000ull) return false;
     }
     return false;
 }
@@ -157,8 +161,11 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
     return remote;
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {  // `bar` is a cluster address
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrival on a barrier of either CTA (`bar` is a cluster address), for consumers of tensor memory: what it orders are
+// loads that tcgen05.wait has completed.  A release at cluster scope would wait for every other access of the warp as
+// well, 1.2 us per block of k.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
     float v;
