@@ -83,7 +83,7 @@ struct MatmulPlan {
 MatmulPlan plan_matmul(long long M, long long N, int n_kb) {
     const long long sms = sm_count();
     const long long big = ((M + MMR_M - 1) / MMR_M) * ((N + MMR_N - 1) / MMR_N);
-    if (M > 64 && big >= sms / 2) return {0, 1, 128, 128};
+    if (M > 64 && big >= sms / 2) return {0, 1, 128, 64};
     const int T = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const long long tiles = ((N + 127) / 128) * ((M + T - 1) / T);
     int S = 1;

@@ -46,18 +46,24 @@ __device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) { return make_
 // CTAs that is a third less to read from L2 per product.  Persistent: one pair per two SMs walks the tiles.
 //
 // Lane = row: a thread owns one row's sums of 128 columns, and both scales of a block are one factor for all of them.
-// A warp of its own fetches the factors ahead of their use.  Results leave through shared memory and bulk stores of
-// 32 rows x 128 bytes per warp, so that the sums' registers are free for the next tile at once.
+// The product of a block of k is issued as two of 128 columns, each with two buffers of tensor memory of its own: a
+// buffer's way from its product through the other CTA's sums back to the next product is a chain of latencies (product,
+// commit, read back, arrival on the other SM), and with halves the tensor cores have more to do meanwhile.  Scales are
+// copied ahead of their use by a warp of its own.  Results leave through shared memory and bulk stores of 32 rows x 128
+// bytes per warp, so that the sums' registers are free for the next tile at once.
 // ---------------------------------------------------------------------------------------------
-constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;  // a pair's tile
+constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;        // a pair's tile
 constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
-constexpr int MMR_THREADS = 384;  // warps 0-7 sums, 8 copies, 9 products, 10 factors
-constexpr int MMR_FACTORS = 8;    // blocks of factors in flight
-constexpr int MMR_OUT = MMR_STAGES * MMR_STAGE, MMR_BIAS = MMR_OUT + 8 * 2 * 4096, MMR_FACT = MMR_BIAS + 8 * 512,
-              MMR_BARS = MMR_FACT + MMR_FACTORS * 1024, MMR_SMEM = MMR_BARS + 256 + 1024;
+constexpr int MMR_WARPS = 8, MMR_COLS = 128;                   // warps that hold sums, columns of each
+constexpr int MMR_THREADS = 32 * MMR_WARPS + 128;              // warp 8 copies, 9 and 10 products, 11 scales
+constexpr int MMR_SLOTS = 8, MMR_SLOT = 576;                   // blocks of scales in flight: 128 of x, two of w
+constexpr int MMR_OUT = MMR_STAGES * MMR_STAGE, MMR_BIAS = MMR_OUT + MMR_WARPS * 8192,
+              MMR_SCALES = MMR_BIAS + MMR_WARPS * MMR_COLS * 4, MMR_BARS = MMR_SCALES + MMR_SLOTS * MMR_SLOT,
+              MMR_SMEM = MMR_BARS + 512 + 1024;
 // Registers: 168 a thread at launch (384 threads); the four helper warps give 96 of theirs to the eight others.
 constexpr int MMR_REGS_SUMS = 216, MMR_REGS_HELP = 72;
-static_assert(256 * MMR_REGS_SUMS + 128 * MMR_REGS_HELP <= 384 * 168, "more registers than the CTA has");
+static_assert(32 * MMR_WARPS * MMR_REGS_SUMS + 128 * MMR_REGS_HELP <= MMR_THREADS * 168, "more registers than the CTA has");
+static_assert(MMR_SMEM <= 227 * 1024, "more shared memory than a CTA has");
 
 template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMR_THREADS, 1)
     matmul_fp8_rows_kernel(const __grid_constant__ MatmulParams p) {
@@ -65,20 +71,20 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t base = smem_u32(smem), bars = base + MMR_BARS;
     // full, taken: the even CTA's count for both; the others are each CTA's own
-    const uint32_t full = bars, empty = full + 8 * MMR_STAGES, done = empty + 8 * MMR_STAGES, taken = done + 16,
-                   fready = taken + 16, fused = fready + 8 * MMR_FACTORS, last = fused + 8 * MMR_FACTORS;
-    static_assert(8 * (2 * MMR_STAGES + 4 + 2 * MMR_FACTORS + 1) + 4 <= 256, "room for the barriers");
+    const uint32_t full = bars, empty = full + 8 * MMR_STAGES, done = empty + 8 * MMR_STAGES, taken = done + 32,
+                   scaled = taken + 32, used = scaled + 8 * MMR_SLOTS, last = used + 8 * MMR_SLOTS;
+    static_assert(8 * (2 * MMR_STAGES + 8 + 2 * MMR_SLOTS + 1) + 4 <= 512, "room for the barriers");
     volatile uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + (last + 8 - base));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, 16); }
-        for (int f = 0; f < MMR_FACTORS; ++f) { mbar_init(fready + 8 * f, 1); mbar_init(fused + 8 * f, 8); }
-        mbar_init(last, 1);
+        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 2); }
+        for (int b = 0; b < 4; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, MMR_WARPS); }
+        for (int f = 0; f < MMR_SLOTS; ++f) { mbar_init(scaled + 8 * f, 32); mbar_init(used + 8 * f, MMR_WARPS); }
+        mbar_init(last, 2);
         fence_barrier_init();
     }
-    if (warp == 9) tmem_alloc<2>(smem_u32(const_cast<uint32_t*>(tmem_at)), 512);
+    if (warp == MMR_WARPS + 1) tmem_alloc<2>(smem_u32(const_cast<uint32_t*>(tmem_at)), 512);
     tc_fence_before();
     __syncthreads();
     cluster_sync();
@@ -87,129 +93,135 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     const int tiles = p.m_tiles * p.n_tiles, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     bool ok = true;
 
-    if (warp >= 8) {
+    if (warp >= MMR_WARPS) {
         regs_down<MMR_REGS_HELP>();
-        if (warp == 8 && lane == 0) {
-            prefetch_map(&p.x_map);
-            prefetch_map(&p.w_map);
+        if (warp == MMR_WARPS) {
             const uint32_t full0 = cluster_addr(full, 0);
             uint32_t it = 0;
             for (int t = pair; ok && t < tiles; t += pairs) {
-                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N + (int)rank * 128;
+                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N + (int)rank * 64;
                 for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
                     const uint32_t s = it % MMR_STAGES, round = it / MMR_STAGES;
-                    if (round > 0 && !mbar_wait_limit(empty + 8 * s, (round - 1) & 1)) { ok = false; break; }
-                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * MMR_STAGE);
-                    tma_load_2d_pair(base + s * MMR_STAGE, &p.x_map, full0 + 8 * s, kb * MM_TILE_K, m0);
-                    tma_load_2d_pair(base + s * MMR_STAGE + MMR_A, &p.w_map, full0 + 8 * s, kb * MM_TILE_K, n0);
+                    if (round > 0 && !(ok = mbar_wait_warp(false, empty + 8 * s, (round - 1) & 1))) break;
+                    if (elect_one()) {
+                        const uint32_t at = base + s * MMR_STAGE, bar = full0 + 8 * s;
+                        if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * MMR_STAGE);
+                        tma_load_2d_pair(at, &p.x_map, bar, kb * MM_TILE_K, m0);
+                        tma_load_2d_pair(at + MMR_A, &p.w_map, bar, kb * MM_TILE_K, n0);
+                        tma_load_2d_pair(at + MMR_A + MMR_A / 2, &p.w_map, bar, kb * MM_TILE_K, n0 + 128);
+                    }
                 }
             }
             // no copy outlives the pair: the last rounds' products are done (both CTAs are told), or time is given
             const uint32_t left = it < (uint32_t)MMR_STAGES ? it : (uint32_t)MMR_STAGES;
             for (uint32_t i = it - left; ok && i < it; ++i) ok = mbar_wait_limit(empty + 8 * (i % MMR_STAGES), (i / MMR_STAGES) & 1);
             if (!ok) wait_ns(1000000);
-        } else if (warp == 9 && lane == 0 && rank == 0) {
-            constexpr uint32_t idesc = fp8_idesc(MMR_M, MMR_N);
-            uint32_t it = 0;
-            for (int t = pair; ok && t < tiles; t += pairs) {
-                for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
-                    const uint32_t s = it % MMR_STAGES, b = it & 1;
-                    if (it >= 2 && !mbar_wait_limit(taken + 8 * b, ((it >> 1) - 1) & 1)) { ok = false; break; }
-                    if (!mbar_wait_limit(full + 8 * s, (it / MMR_STAGES) & 1)) { ok = false; break; }
+        } else if (warp <= MMR_WARPS + 2) {
+            // one warp for each half of the columns: issuing a block's products and handing its barriers on takes a warp
+            // about as long as the products themselves
+            if (rank == 0) {
+                constexpr uint32_t idesc = fp8_idesc(MMR_M, 128);
+                const uint32_t half = warp - (MMR_WARPS + 1);
+                const uint32_t total = (uint32_t)((tiles - pair + pairs - 1) / pairs) * (uint32_t)p.n_kb;
+                const uint32_t my_taken = taken + 8 * half, my_done = done + 8 * half, d = tmem + half * 128;
+                bool filled = false, freed = true;
+                for (uint32_t it = 0; it < total; ++it) {
+                    const uint32_t s = it % MMR_STAGES, b = it & 1, ni = it + 1;
+                    const uint64_t x = smem_operand(base + s * MMR_STAGE),
+                                   w = smem_operand(base + s * MMR_STAGE + MMR_A + half * (MMR_A / 2));
+                    if (!(ok = mbar_wait_warp(filled, full + 8 * s, (it / MMR_STAGES) & 1))) break;
+                    if (it >= 2 && !(ok = mbar_wait_warp(freed, my_taken + 16 * b, ((it >> 1) - 1) & 1))) break;
                     tc_fence_after();
-                    const uint64_t x = smem_operand(base + s * MMR_STAGE), w = smem_operand(base + s * MMR_STAGE + MMR_A);
+                    filled = mbar_peek(full + 8 * (ni % MMR_STAGES), (ni / MMR_STAGES) & 1);
+                    freed = mbar_peek(my_taken + 16 * (ni & 1), ((ni >> 1) - 1) & 1);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc_mma_fp8_pair(tmem + b * MMR_N, x + 2 * k, w + 2 * k, idesc, k > 0);
-                    tc_commit_pair(empty + 8 * s);
-                    tc_commit_pair(done + 8 * b);
+                        for (int k = 0; k < 4; ++k) tc_mma_fp8_pair(d + b * 256, x + 2 * k, w + 2 * k, idesc, k > 0);
+                        tc_commit_pair(my_done + 16 * b);
+                        tc_commit_pair(empty + 8 * s);
+                    }
+                    __syncwarp();
                 }
+                if (elect_one()) tc_commit_group2(last);  // no product outlives the pair
+                ok &= mbar_wait_limit(last, 0);
             }
-            tc_commit_group2(last);  // no product outlives the pair
-            ok &= mbar_wait_limit(last, 0);
-        } else if (warp == 10) {
-            // factors of block kb: scale of the row x scale of the weight's block, for 128 rows x two halves of columns
-            float* out = reinterpret_cast<float*>(smem + MMR_FACT);
+        } else {
             uint32_t it = 0;
             for (int t = pair; ok && t < tiles; t += pairs) {
-                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N;
+                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + lane, n0 = (t / p.m_tiles) * MMR_N + (lane & 1) * 128;
+                const float* w = p.w_scales + (long long)(n0 < p.N ? n0 / 128 : 0) * p.ws_row;
                 const float* xs[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int m = m0 + 32 * i + lane;
-                    xs[i] = p.x_scales + (long long)(m < p.M ? m : 0) * p.xs_row;
-                }
-                const float* w0 = p.w_scales + (long long)(n0 / 128) * p.ws_row;
-                const float* w1 = n0 + 128 < p.N ? w0 + p.ws_row : w0;
-                constexpr int AHEAD = 2;  // blocks fetched together
-                for (int kb0 = 0; ok && kb0 < p.n_kb; kb0 += AHEAD) {
-                    float x[AHEAD][4], w[AHEAD][2];
+                for (int i = 0; i < 4; ++i) xs[i] = p.x_scales + (long long)(m0 + 32 * i < p.M ? m0 + 32 * i : 0) * p.xs_row;
+                for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
+                    const uint32_t f = it % MMR_SLOTS, round = it / MMR_SLOTS;
+                    if (round > 0 && !mbar_wait_limit(used + 8 * f, (round - 1) & 1)) { ok = false; break; }
+                    const uint32_t slot = base + MMR_SCALES + f * MMR_SLOT + lane * 4;
 #pragma unroll
-                    for (int a = 0; a < AHEAD; ++a) {
-                        const long long kb = kb0 + a < p.n_kb ? kb0 + a : kb0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[a][i] = xs[i][kb * p.xs_blk];
-                        w[a][0] = w0[kb * p.ws_blk];
-                        w[a][1] = w1[kb * p.ws_blk];
+                    for (int i = 0; i < 4; ++i) {
+                        copy_4(slot + 128 * i, xs[i]);
+                        xs[i] += p.xs_blk;
                     }
-#pragma unroll
-                    for (int a = 0; a < AHEAD; ++a) {
-                        if (kb0 + a >= p.n_kb) break;
-                        const uint32_t f = it % MMR_FACTORS, round = it / MMR_FACTORS;
-                        if (round > 0 && !mbar_wait_limit(fused + 8 * f, (round - 1) & 1)) { ok = false; break; }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            out[f * 256 + 32 * i + lane] = x[a][i] * w[a][0];
-                            out[f * 256 + 128 + 32 * i + lane] = x[a][i] * w[a][1];
-                        }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(fready + 8 * f);
-                        ++it;
-                    }
+                    if (lane < 2) copy_4(slot + 512, w);
+                    w += p.ws_blk;
+                    copies_arrive(scaled + 8 * f);
                 }
+                ok = __all_sync(0xffffffffu, ok);
             }
+            copies_wait();
         }
     } else {
         regs_up<MMR_REGS_SUMS>();
-        const int half = warp >> 2, quarter = warp & 3;
+        const int quarter = warp & 3, half = warp >> 2, col0 = half * MMR_COLS;
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
-        const uint32_t taken0 = cluster_addr(taken, 0);
-        float* my_bias = reinterpret_cast<float*>(smem + MMR_BIAS) + warp * 128;
-        const float* my_factor = reinterpret_cast<const float*>(smem + MMR_FACT) + half * 128 + quarter * 32 + lane;
-        const uint32_t out = base + MMR_OUT + warp * 8192;
-        uint8_t* const out_row = smem + MMR_OUT + warp * 8192 + lane * 128;
+        const uint32_t taken0 = cluster_addr(taken, 0) + 8 * half, my_done = done + 8 * half;
+        float* my_bias = reinterpret_cast<float*>(smem + MMR_BIAS) + warp * MMR_COLS;
+        const float* my_x = reinterpret_cast<const float*>(smem + MMR_SCALES) + quarter * 32 + lane;
+        const float* my_w = reinterpret_cast<const float*>(smem + MMR_SCALES) + 128 + half;
         uint32_t it = 0;
+        bool scales_here = false, sums_here = false;  // peeked
         for (int t = pair; ok && t < tiles; t += pairs) {
-            const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + quarter * 32, n0 = (t / p.m_tiles) * MMR_N + half * 128;
-            __syncwarp();
+            const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + quarter * 32, n0 = (t / p.m_tiles) * MMR_N + col0;
+            float2 acc[MMR_COLS / 2];
+            if (p.bias != nullptr) {  // the sums start from the bias
+                __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) my_bias[i * 32 + lane] = load_bias(p, n0 + i * 32 + lane);
-            __syncwarp();
-            float2 acc[64];  // the sums start from the bias
+                for (int i = 0; i < MMR_COLS; i += 32) my_bias[i + lane] = load_bias(p, n0 + i + lane);
+                __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float4 v = *reinterpret_cast<const float4*>(my_bias + 4 * j);
-                acc[2 * j] = make_float2(v.x, v.y);
-                acc[2 * j + 1] = make_float2(v.z, v.w);
+                for (int j = 0; j < MMR_COLS / 4; ++j) {
+                    const float4 v = *reinterpret_cast<const float4*>(my_bias + 4 * j);
+                    acc[2 * j] = make_float2(v.x, v.y);
+                    acc[2 * j + 1] = make_float2(v.z, v.w);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < MMR_COLS / 2; ++j) acc[j] = make_float2(0.f, 0.f);
             }
             for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
-                const uint32_t b = it & 1, f = it % MMR_FACTORS;
-                if (!mbar_wait_limit(fready + 8 * f, (it / MMR_FACTORS) & 1)) { ok = false; break; }
-                const float factor = my_factor[f * 256];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(fused + 8 * f);
-                if (!mbar_wait_limit(done + 8 * b, (it >> 1) & 1)) { ok = false; break; }
+                const uint32_t b = it & 1, f = it % MMR_SLOTS;
+                if (!(ok = mbar_wait_warp(sums_here, my_done + 16 * b, (it >> 1) & 1))) break;
                 tc_fence_after();
-                const float2 s = make_float2(factor, factor);
                 uint32_t r[2][32];
-                tmem_ld<32>(at + b * MMR_N, r[0]);
+                tmem_ld<32>(at + b * 256, r[0]);
+                // while that comes: this row's factor, scale of the row x scale of the weight's block
+                if (!(ok = mbar_wait_warp(scales_here, scaled + 8 * f, (it / MMR_SLOTS) & 1))) break;
+                const float factor = my_x[f * (MMR_SLOT / 4)] * my_w[f * (MMR_SLOT / 4)];
+                const float2 s = make_float2(factor, factor);
+                const uint32_t ni = it + 1, nf = ni % MMR_SLOTS;
+                scales_here = mbar_peek(scaled + 8 * nf, (ni / MMR_SLOTS) & 1);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     tc_wait_ld(r[c & 1]);
-                    if (c < 3) tmem_ld<32>(at + b * MMR_N + 32 * (c + 1), r[(c + 1) & 1]);
+                    if (c < 3) tmem_ld<32>(at + b * 256 + 32 * (c + 1), r[(c + 1) & 1]);
                     else {  // all read: the buffer may be written again
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(taken0 + 8 * b);
+                        if (lane == 0) {
+                            mbar_arrive_cluster(taken0 + 16 * b);
+                            mbar_arrive(used + 8 * f);
+                        }
+                        sums_here = mbar_peek(my_done + 16 * (ni & 1), (ni >> 1) & 1);
                     }
 #pragma unroll
                     for (int j = 0; j < 16; ++j) fma_pair(acc[16 * c + j], as_pair(r[c & 1][2 * j], r[c & 1][2 * j + 1]), s);
@@ -218,12 +230,12 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
             if (!ok || m0 >= p.M || n0 >= p.N) continue;
             // 128 bytes of each row at a time; 16-byte piece c of row r lies at c ^ (r & 7), where a bulk store in the
             // 128-byte swizzle looks for it, and eight lanes' pieces in eight different banks
-            constexpr int V = 16 / sizeof(T), COLS = 8 * V, CHUNKS = 128 / COLS;
+            constexpr int V = 16 / sizeof(T), COLS = 8 * V, CHUNKS = MMR_COLS / COLS;
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c) {
+                uint8_t* const buf = smem + MMR_OUT + warp * 8192 + (c & 1) * 4096;
                 if (lane == 0) tma_wait_read<1>();  // the store that read this buffer before
                 __syncwarp();
-                uint8_t* row = out_row + (c & 1) * 4096;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     float v[V];
@@ -232,24 +244,24 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                         v[i] = acc[(c * COLS + q * V + i) / 2].x;
                         v[i + 1] = acc[(c * COLS + q * V + i) / 2].y;
                     }
-                    store_elems<T, V>(reinterpret_cast<T*>(row + ((q ^ (lane & 7)) << 4)), v);
+                    store_elems<T, V>(reinterpret_cast<T*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)), v);
                 }
                 if (p.y_vec) {
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        if (n0 + c * COLS < p.N) tma_store_2d(&p.y_map, out + (c & 1) * 4096, n0 + c * COLS, m0);
+                        if (n0 + c * COLS < p.N) tma_store_2d(&p.y_map, smem_u32(buf), n0 + c * COLS, m0);
                         tma_commit();
                     }
                 } else {  // rows of y on any boundary: each row's piece by consecutive lanes
                     __syncwarp();
                     const int rows = p.M - m0 < 32 ? p.M - m0 : 32, cols = p.N - n0 - c * COLS;
                     for (int r = 0; r < rows; ++r) {
-                        const uint8_t* src = smem + MMR_OUT + warp * 8192 + (c & 1) * 4096 + r * 128;
                         T* dst = static_cast<T*>(p.y) + (long long)(m0 + r) * p.y_stride + n0 + c * COLS;
 #pragma unroll
                         for (int i = lane; i < COLS; i += 32)
-                            if (i < cols) dst[i] = *reinterpret_cast<const T*>(src + (((i / V) ^ (r & 7)) << 4) + (i % V) * sizeof(T));
+                            if (i < cols)
+                                dst[i] = *reinterpret_cast<const T*>(buf + r * 128 + (((i / V) ^ (r & 7)) << 4) + (i % V) * sizeof(T));
                     }
                 }
             }
@@ -262,7 +274,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     __syncthreads();
     cluster_sync();
     tc_fence_after();
-    if (warp == 9) tmem_free<2>(tmem, 512);
+    if (warp == MMR_WARPS + 1) tmem_free<2>(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------------------------

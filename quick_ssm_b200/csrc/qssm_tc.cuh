@@ -5,8 +5,20 @@
 
 namespace qssm {
 
-// Waits until the barrier's phase `parity` has completed; gives up after about two seconds.  The timer is not read in
-// the first tries: reading it takes longer than most waits (about a microsecond).
+// Has the barrier's phase `parity` completed?  Does not wait.  A wait that is over already still takes 80 to 180 cycles
+// from the test to the branch on it, so loops that hand work on test the next barrier ahead of their present work.
+__device__ __forceinline__ bool mbar_peek(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Waits until that phase has completed; gives up after about two seconds.
 __device__ __forceinline__ bool mbar_wait_limit(uint32_t bar, uint32_t parity) {
 #pragma unroll 1
     for (int it = 0; it < 256; ++it)
@@ -18,6 +30,11 @@ __device__ __forceinline__ bool mbar_wait_limit(uint32_t bar, uint32_t parity) {
         if ((it & 255u) == 255u && global_timer_ns() - t0 > 2000000000ull) return false;
     }
     return false;
+}
+// The same for a whole converged warp that has peeked before: all of it goes on or none.
+__device__ __forceinline__ bool mbar_wait_warp(bool peeked, uint32_t bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, peeked)) return true;
+    return __all_sync(0xffffffffu, mbar_wait_limit(bar, parity));
 }
 __device__ __forceinline__ void wait_ns(unsigned long long ns) {
     const unsigned long long t0 = global_timer_ns();
@@ -50,6 +67,16 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
                  "r"(src), "r"(c0), "r"(c1)
                  : "memory");
 }
+
+// Four bytes from global to shared memory behind the warp's back; `copies_arrive` arrives on the barrier for this thread
+// once its copies so far have landed (the barrier's count includes the thread).
+__device__ __forceinline__ void copy_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ---- tensor memory ----------------------------------------------------------------------------
 // G = 1: one CTA; 2: both CTAs of a pair, each with a whole warp.
@@ -114,6 +141,14 @@ template <> __device__ __forceinline__ void tmem_ld<32>(uint32_t at, uint32_t (&
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(at));
+}
+
+// One lane of a converged warp, always the same.  Products and commits are issued under it by a warp that runs its loop as
+// a whole: their operands then stay in uniform registers (under `lane == 0` each product took 70 cycles to issue).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
 }
 
 // ---- products -----------------------------------------------------------------------------------
