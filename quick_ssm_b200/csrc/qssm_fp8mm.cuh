@@ -46,23 +46,24 @@ __device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) { return make_
 // CTAs that is a third less to read from L2 per product.  Persistent: one pair per two SMs walks the tiles.
 //
 // Lane = row: a thread owns one row's sums of 128 columns, and both scales of a block are one factor for all of them.
-// The product of a block of k is issued as two of 128 columns, each with two buffers of tensor memory of its own: a
-// buffer's way from its product through the other CTA's sums back to the next product is a chain of latencies (product,
-// commit, read back, arrival on the other SM), and with halves the tensor cores have more to do meanwhile.  Scales are
-// copied ahead of their use by a warp of its own.  Results leave through shared memory and bulk stores of 32 rows x 128
-// bytes per warp, so that the sums' registers are free for the next tile at once.
+// The product of a block of k is issued as two of 128 columns, each with two buffers of tensor memory of its own.  What
+// bounds the kernel is the way of a buffer from its product through both CTAs' sums back to the next product, a chain of
+// latencies (issue, commit, test, read back, arrival on the other SM, test; a branch alone is 40 cycles).  So each
+// buffer has an issuing warp of its own, the scales arrive on the same barrier as the tiles, and the sums' loop has no
+// other wait than the one for its product.  Results leave through shared memory and bulk stores of 32 rows x 128 bytes
+// per warp, so that the sums' registers are free for the next tile at once.
 // ---------------------------------------------------------------------------------------------
 constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;        // a pair's tile
 constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
 constexpr int MMR_WARPS = 8, MMR_COLS = 128;                   // warps that hold sums, columns of each
-constexpr int MMR_THREADS = 32 * MMR_WARPS + 128;              // warp 8 copies, 9 and 10 products, 11 scales
+constexpr int MMR_THREADS = 32 * MMR_WARPS + 256;              // warp 8 copies, 9 to 12 products, 13 scales
 constexpr int MMR_SLOTS = 8, MMR_SLOT = 576;                   // blocks of scales in flight: 128 of x, two of w
 constexpr int MMR_OUT = MMR_STAGES * MMR_STAGE, MMR_BIAS = MMR_OUT + MMR_WARPS * 8192,
               MMR_SCALES = MMR_BIAS + MMR_WARPS * MMR_COLS * 4, MMR_BARS = MMR_SCALES + MMR_SLOTS * MMR_SLOT,
               MMR_SMEM = MMR_BARS + 512 + 1024;
-// Registers: 168 a thread at launch (384 threads); the four helper warps give 96 of theirs to the eight others.
-constexpr int MMR_REGS_SUMS = 216, MMR_REGS_HELP = 72;
-static_assert(32 * MMR_WARPS * MMR_REGS_SUMS + 128 * MMR_REGS_HELP <= MMR_THREADS * 168, "more registers than the CTA has");
+// Registers: 128 a thread at launch (512 threads); the eight helper warps give 80 of theirs to the eight others.
+constexpr int MMR_REGS_SUMS = 208, MMR_REGS_HELP = 48;
+static_assert(256 * MMR_REGS_SUMS + 256 * MMR_REGS_HELP <= MMR_THREADS * 128, "more registers than the CTA has");
 static_assert(MMR_SMEM <= 227 * 1024, "more shared memory than a CTA has");
 
 template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMR_THREADS, 1)
@@ -70,7 +71,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t base = smem_u32(smem), bars = base + MMR_BARS;
-    // full, taken: the even CTA's count for both; the others are each CTA's own
+    // full, taken: the even CTA's count for both; the others are each CTA's own.  Buffer b = 2 * (block & 1) + half.
     const uint32_t full = bars, empty = full + 8 * MMR_STAGES, done = empty + 8 * MMR_STAGES, taken = done + 32,
                    scaled = taken + 32, used = scaled + 8 * MMR_SLOTS, last = used + 8 * MMR_SLOTS;
     static_assert(8 * (2 * MMR_STAGES + 8 + 2 * MMR_SLOTS + 1) + 4 <= 512, "room for the barriers");
@@ -78,10 +79,10 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 2); }
+        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 2); }  // empty: both halves
         for (int b = 0; b < 4; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, MMR_WARPS); }
         for (int f = 0; f < MMR_SLOTS; ++f) { mbar_init(scaled + 8 * f, 32); mbar_init(used + 8 * f, MMR_WARPS); }
-        mbar_init(last, 2);
+        mbar_init(last, 4);
         fence_barrier_init();
     }
     if (warp == MMR_WARPS + 1) tmem_alloc<2>(smem_u32(const_cast<uint32_t*>(tmem_at)), 512);
@@ -91,6 +92,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
     const int tiles = p.m_tiles * p.n_tiles, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t total = pair < tiles ? (uint32_t)((tiles - pair + pairs - 1) / pairs) * (uint32_t)p.n_kb : 0;
     bool ok = true;
 
     if (warp >= MMR_WARPS) {
@@ -102,7 +104,8 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                 const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N + (int)rank * 64;
                 for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
                     const uint32_t s = it % MMR_STAGES, round = it / MMR_STAGES;
-                    if (round > 0 && !(ok = mbar_wait_warp(false, empty + 8 * s, (round - 1) & 1))) break;
+                    if (round > 0) ok = mbar_wait_limit(empty + 8 * s, (round - 1) & 1);
+                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
                     if (elect_one()) {
                         const uint32_t at = base + s * MMR_STAGE, bar = full0 + 8 * s;
                         if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * MMR_STAGE);
@@ -116,36 +119,34 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
             const uint32_t left = it < (uint32_t)MMR_STAGES ? it : (uint32_t)MMR_STAGES;
             for (uint32_t i = it - left; ok && i < it; ++i) ok = mbar_wait_limit(empty + 8 * (i % MMR_STAGES), (i / MMR_STAGES) & 1);
             if (!ok) wait_ns(1000000);
-        } else if (warp <= MMR_WARPS + 2) {
-            // one warp for each half of the columns: issuing a block's products and handing its barriers on takes a warp
-            // about as long as the products themselves
-            if (rank == 0) {
+        } else if (warp <= MMR_WARPS + 4) {
+            if (rank == 0) {  // warp 9 + b issues the products of buffer b: every second block's, of one half of the columns
                 constexpr uint32_t idesc = fp8_idesc(MMR_M, 128);
-                const uint32_t half = warp - (MMR_WARPS + 1);
-                const uint32_t total = (uint32_t)((tiles - pair + pairs - 1) / pairs) * (uint32_t)p.n_kb;
-                const uint32_t my_taken = taken + 8 * half, my_done = done + 8 * half, d = tmem + half * 128;
-                bool filled = false, freed = true;
-                for (uint32_t it = 0; it < total; ++it) {
-                    const uint32_t s = it % MMR_STAGES, b = it & 1, ni = it + 1;
+                const uint32_t b = warp - (MMR_WARPS + 1), half = b & 1;
+                const uint32_t my_taken = taken + 8 * b, my_done = done + 8 * b, d = tmem + b * 128;
+                uint32_t round = 0;
+                for (uint32_t it = b >> 1; it < total; it += 2, ++round) {
+                    const uint32_t s = it % MMR_STAGES;
                     const uint64_t x = smem_operand(base + s * MMR_STAGE),
                                    w = smem_operand(base + s * MMR_STAGE + MMR_A + half * (MMR_A / 2));
-                    if (!(ok = mbar_wait_warp(filled, full + 8 * s, (it / MMR_STAGES) & 1))) break;
-                    if (it >= 2 && !(ok = mbar_wait_warp(freed, my_taken + 16 * b, ((it >> 1) - 1) & 1))) break;
+                    ok = mbar_wait_limit(full + 8 * s, (it / MMR_STAGES) & 1);
+                    if (round > 0) ok &= mbar_wait_limit(my_taken, (round - 1) & 1);
+                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
                     tc_fence_after();
-                    filled = mbar_peek(full + 8 * (ni % MMR_STAGES), (ni / MMR_STAGES) & 1);
-                    freed = mbar_peek(my_taken + 16 * (ni & 1), ((ni >> 1) - 1) & 1);
                     if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) tc_mma_fp8_pair(d + b * 256, x + 2 * k, w + 2 * k, idesc, k > 0);
-                        tc_commit_pair(my_done + 16 * b);
+                        for (int k = 0; k < 4; ++k) tc_mma_fp8_pair(d, x + 2 * k, w + 2 * k, idesc, k > 0);
+                        tc_commit_pair(my_done);
                         tc_commit_pair(empty + 8 * s);
                     }
                     __syncwarp();
                 }
                 if (elect_one()) tc_commit_group2(last);  // no product outlives the pair
                 ok &= mbar_wait_limit(last, 0);
+                // nor an arrival from the other CTA: it would land in the barriers of the next kernel on this SM
+                if (round > 0) ok &= mbar_wait_limit(my_taken, (round - 1) & 1);
             }
-        } else {
+        } else if (warp == MMR_WARPS + 5) {
             uint32_t it = 0;
             for (int t = pair; ok && t < tiles; t += pairs) {
                 const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + lane, n0 = (t / p.m_tiles) * MMR_N + (lane & 1) * 128;
@@ -155,7 +156,8 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                 for (int i = 0; i < 4; ++i) xs[i] = p.x_scales + (long long)(m0 + 32 * i < p.M ? m0 + 32 * i : 0) * p.xs_row;
                 for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
                     const uint32_t f = it % MMR_SLOTS, round = it / MMR_SLOTS;
-                    if (round > 0 && !mbar_wait_limit(used + 8 * f, (round - 1) & 1)) { ok = false; break; }
+                    if (round > 0) ok = mbar_wait_limit(used + 8 * f, (round - 1) & 1);
+                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
                     const uint32_t slot = base + MMR_SCALES + f * MMR_SLOT + lane * 4;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -166,7 +168,6 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                     w += p.ws_blk;
                     copies_arrive(scaled + 8 * f);
                 }
-                ok = __all_sync(0xffffffffu, ok);
             }
             copies_wait();
         }
@@ -179,7 +180,6 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
         const float* my_x = reinterpret_cast<const float*>(smem + MMR_SCALES) + quarter * 32 + lane;
         const float* my_w = reinterpret_cast<const float*>(smem + MMR_SCALES) + 128 + half;
         uint32_t it = 0;
-        bool scales_here = false, sums_here = false;  // peeked
         for (int t = pair; ok && t < tiles; t += pairs) {
             const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + quarter * 32, n0 = (t / p.m_tiles) * MMR_N + col0;
             float2 acc[MMR_COLS / 2];
@@ -198,18 +198,16 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
 #pragma unroll
                 for (int j = 0; j < MMR_COLS / 2; ++j) acc[j] = make_float2(0.f, 0.f);
             }
-            for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
+            for (int kb = 0; ok && kb < p.n_kb; ++kb, ++it) {
                 const uint32_t b = it & 1, f = it % MMR_SLOTS;
-                if (!(ok = mbar_wait_warp(sums_here, my_done + 16 * b, (it >> 1) & 1))) break;
+                ok = mbar_wait_limit(my_done + 16 * b, (it >> 1) & 1);
                 tc_fence_after();
                 uint32_t r[2][32];
                 tmem_ld<32>(at + b * 256, r[0]);
                 // while that comes: this row's factor, scale of the row x scale of the weight's block
-                if (!(ok = mbar_wait_warp(scales_here, scaled + 8 * f, (it / MMR_SLOTS) & 1))) break;
+                ok &= mbar_wait_limit(scaled + 8 * f, (it / MMR_SLOTS) & 1);
                 const float factor = my_x[f * (MMR_SLOT / 4)] * my_w[f * (MMR_SLOT / 4)];
                 const float2 s = make_float2(factor, factor);
-                const uint32_t ni = it + 1, nf = ni % MMR_SLOTS;
-                scales_here = mbar_peek(scaled + 8 * nf, (ni / MMR_SLOTS) & 1);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     tc_wait_ld(r[c & 1]);
@@ -217,11 +215,10 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                     else {  // all read: the buffer may be written again
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) {
+                        if (lane == 0 && ok) {
                             mbar_arrive_cluster(taken0 + 16 * b);
                             mbar_arrive(used + 8 * f);
                         }
-                        sums_here = mbar_peek(my_done + 16 * (ni & 1), (ni >> 1) & 1);
                     }
 #pragma unroll
                     for (int j = 0; j < 16; ++j) fma_pair(acc[16 * c + j], as_pair(r[c & 1][2 * j], r[c & 1][2 * j + 1]), s);

@@ -5,36 +5,28 @@
 
 namespace qssm {
 
-// Has the barrier's phase `parity` completed?  Does not wait.  A wait that is over already still takes 80 to 180 cycles
-// from the test to the branch on it, so loops that hand work on test the next barrier ahead of their present work.
-__device__ __forceinline__ bool mbar_peek(uint32_t bar, uint32_t parity) {
+// Waits until the barrier's phase `parity` has completed; gives up after two wraps of the low half of the clock (two to
+// seven seconds).  One loop in PTX with one branch in front of a wait that is over: a branch costs a lone warp 40 to 50
+// cycles here, and these waits stand in chains that bound a kernel.
+__device__ __forceinline__ bool mbar_wait_limit(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .u32 t, c;\n\t"
+        "mov.u32 t, %%clock_hi;\n\t"
+        "AGAIN_%=:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra OVER_%=;\n\t"
+        "mov.u32 c, %%clock_hi;\n\t"
+        "sub.u32 c, c, t;\n\t"
+        "setp.lt.u32 p, c, 2;\n\t"
+        "@p bra AGAIN_%=;\n\t"
+        "setp.ne.u32 p, c, c;\n\t"
+        "OVER_%=:\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
     return ok != 0;
-}
-// Waits until that phase has completed; gives up after about two seconds.
-__device__ __forceinline__ bool mbar_wait_limit(uint32_t bar, uint32_t parity) {
-#pragma unroll 1
-    for (int it = 0; it < 256; ++it)
-        if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = global_timer_ns();
-#pragma unroll 1
-    for (uint32_t it = 0; it < (1u << 28); ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 255u) == 255u && global_timer_ns() - t0 > 2000000000ull) return false;
-    }
-    return false;
-}
-// The same for a whole converged warp that has peeked before: all of it goes on or none.
-__device__ __forceinline__ bool mbar_wait_warp(bool peeked, uint32_t bar, uint32_t parity) {
-    if (__all_sync(0xffffffffu, peeked)) return true;
-    return __all_sync(0xffffffffu, mbar_wait_limit(bar, parity));
 }
 __device__ __forceinline__ void wait_ns(unsigned long long ns) {
     const unsigned long long t0 = global_timer_ns();
