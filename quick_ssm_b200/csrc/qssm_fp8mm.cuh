@@ -57,12 +57,13 @@ constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;        // a pair's tile
 constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
 constexpr int MMR_WARPS = 8, MMR_COLS = 128;                   // warps that hold sums, columns of each
 constexpr int MMR_THREADS = 32 * MMR_WARPS + 256;              // warp 8 copies, 9 to 12 products, 13 scales
-constexpr int MMR_SLOTS = 8, MMR_SLOT = 576;                   // blocks of scales in flight: 128 of x, two of w
+// Scales in flight: slots of four blocks, a block being 128 of x and two of w.
+constexpr int MMR_SLOTS = 4, MMR_GROUP = 4, MMR_BLOCK = 576, MMR_SLOT = MMR_GROUP * MMR_BLOCK;
 constexpr int MMR_OUT = MMR_STAGES * MMR_STAGE, MMR_BIAS = MMR_OUT + MMR_WARPS * 8192,
               MMR_SCALES = MMR_BIAS + MMR_WARPS * MMR_COLS * 4, MMR_BARS = MMR_SCALES + MMR_SLOTS * MMR_SLOT,
               MMR_SMEM = MMR_BARS + 512 + 1024;
-// Registers: 128 a thread at launch (512 threads); the eight helper warps give 80 of theirs to the eight others.
-constexpr int MMR_REGS_SUMS = 208, MMR_REGS_HELP = 48;
+// Registers: 128 a thread at launch (512 threads); the eight helper warps give 88 of theirs to the eight others.
+constexpr int MMR_REGS_SUMS = 216, MMR_REGS_HELP = 40;
 static_assert(256 * MMR_REGS_SUMS + 256 * MMR_REGS_HELP <= MMR_THREADS * 128, "more registers than the CTA has");
 static_assert(MMR_SMEM <= 227 * 1024, "more shared memory than a CTA has");
 
@@ -155,18 +156,18 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
 #pragma unroll
                 for (int i = 0; i < 4; ++i) xs[i] = p.x_scales + (long long)(m0 + 32 * i < p.M ? m0 + 32 * i : 0) * p.xs_row;
                 for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
-                    const uint32_t f = it % MMR_SLOTS, round = it / MMR_SLOTS;
-                    if (round > 0) ok = mbar_wait_limit(used + 8 * f, (round - 1) & 1);
+                    const uint32_t group = it / MMR_GROUP, f = group % MMR_SLOTS, round = group / MMR_SLOTS;
+                    if (it % MMR_GROUP == 0 && round > 0) ok = mbar_wait_limit(used + 8 * f, (round - 1) & 1);
                     if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                    const uint32_t slot = base + MMR_SCALES + f * MMR_SLOT + lane * 4;
+                    const uint32_t at = base + MMR_SCALES + f * MMR_SLOT + (it % MMR_GROUP) * MMR_BLOCK + lane * 4;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        copy_4(slot + 128 * i, xs[i]);
+                        copy_4(at + 128 * i, xs[i]);
                         xs[i] += p.xs_blk;
                     }
-                    if (lane < 2) copy_4(slot + 512, w);
+                    if (lane < 2) copy_4(at + 512, w);
                     w += p.ws_blk;
-                    copies_arrive(scaled + 8 * f);
+                    if (it % MMR_GROUP == MMR_GROUP - 1 || it + 1 == total) copies_arrive(scaled + 8 * f);
                 }
             }
             copies_wait();
@@ -199,30 +200,36 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                 for (int j = 0; j < MMR_COLS / 2; ++j) acc[j] = make_float2(0.f, 0.f);
             }
             for (int kb = 0; ok && kb < p.n_kb; ++kb, ++it) {
-                const uint32_t b = it & 1, f = it % MMR_SLOTS;
-                ok = mbar_wait_limit(my_done + 16 * b, (it >> 1) & 1);
-                tc_fence_after();
-                uint32_t r[2][32];
-                tmem_ld<32>(at + b * 256, r[0]);
-                // while that comes: this row's factor, scale of the row x scale of the weight's block
-                ok &= mbar_wait_limit(scaled + 8 * f, (it / MMR_SLOTS) & 1);
-                const float factor = my_x[f * (MMR_SLOT / 4)] * my_w[f * (MMR_SLOT / 4)];
+                const uint32_t b = it & 1, f = (it / MMR_GROUP) % MMR_SLOTS, d = at + b * 256;
+                if (it % MMR_GROUP == 0) ok = mbar_wait_limit(scaled + 8 * f, (it / (MMR_GROUP * MMR_SLOTS)) & 1);
+                const uint32_t where = f * (MMR_SLOT / 4) + (it % MMR_GROUP) * (MMR_BLOCK / 4);
+                const float factor = my_x[where] * my_w[where];  // scale of the row x scale of the weight's block
                 const float2 s = make_float2(factor, factor);
+                ok &= mbar_wait_limit(my_done + 16 * b, (it >> 1) & 1);
+                tc_fence_after();
+                uint32_t r0[32], r1[32];
+                tmem_ld<32>(d, r0);
+                tmem_ld<32>(d + 32, r1);
+                tc_wait_ld(r0);
+                tc_landed(r1);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tc_wait_ld(r[c & 1]);
-                    if (c < 3) tmem_ld<32>(at + b * 256 + 32 * (c + 1), r[(c + 1) & 1]);
-                    else {  // all read: the buffer may be written again
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0 && ok) {
-                            mbar_arrive_cluster(taken0 + 16 * b);
-                            mbar_arrive(used + 8 * f);
-                        }
-                    }
+                for (int j = 0; j < 16; ++j) fma_pair(acc[j], as_pair(r0[2 * j], r0[2 * j + 1]), s);
+                tmem_ld<32>(d + 64, r0);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) fma_pair(acc[16 * c + j], as_pair(r[c & 1][2 * j], r[c & 1][2 * j + 1]), s);
+                for (int j = 0; j < 16; ++j) fma_pair(acc[16 + j], as_pair(r1[2 * j], r1[2 * j + 1]), s);
+                tmem_ld<32>(d + 96, r1);
+                tc_wait_ld(r0);
+                tc_landed(r1);
+                tc_fence_before();  // all read: the buffer may be written again
+                __syncwarp();
+                if (lane == 0 && ok) {
+                    mbar_arrive_cluster(taken0 + 16 * b);
+                    if (it % MMR_GROUP == MMR_GROUP - 1) mbar_arrive(used + 8 * f);
                 }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) fma_pair(acc[32 + j], as_pair(r0[2 * j], r0[2 * j + 1]), s);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) fma_pair(acc[48 + j], as_pair(r1[2 * j], r1[2 * j + 1]), s);
             }
             if (!ok || m0 >= p.M || n0 >= p.N) continue;
             // 128 bytes of each row at a time; 16-byte piece c of row r lies at c ^ (r & 7), where a bulk store in the

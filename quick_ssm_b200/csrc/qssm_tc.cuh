@@ -102,10 +102,10 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
         "h"((uint16_t)3)
         : "memory");
 }
-// The loads into these registers are done (they are operands, so that nothing that reads them moves in front).
-template <int N> __device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[N]) {
+// Behind a wait for loads: these registers hold their results (as operands, so that nothing that reads them moves in
+// front of the wait).
+template <int N> __device__ __forceinline__ void tc_landed(uint32_t (&r)[N]) {
     static_assert(N % 16 == 0, "sixteen at a time");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < N; i += 16)
         asm volatile(""
@@ -141,6 +141,11 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t yes;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
     return yes != 0;
+}
+
+template <int N> __device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    tc_landed(r);
 }
 
 // ---- products -----------------------------------------------------------------------------------
