@@ -100,7 +100,7 @@ template <typename OUT, int T> int launch_few(const MatmulParams& p, int S, cuda
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)gx, (unsigned)gy);
-    cfg.blockDim = dim3(MMF_THREADS);
+    cfg.blockDim = dim3(Few<T>::THREADS);
     cfg.dynamicSmemBytes = Few<T>::SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

@@ -284,168 +284,176 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
 // ---------------------------------------------------------------------------------------------
 // Few rows: the weight is the first operand.  Tiles of 128 columns of y x T rows (T = 16 to 128), lane = column, so
 // the weight's rows fill the tensor cores' 128 lanes however few rows there are, and k is cut over the S CTAs of a
-// cluster, whose sums are added in rank order through distributed shared memory (each CTA adds T / S of the rows).
+// cluster, whose sums are added in rank order through distributed shared memory (each CTA adds every S-th row).
+// Bound by latencies: a CTA sees few blocks of k, each a copy, a product and a read back.
 // ---------------------------------------------------------------------------------------------
 template <int T> struct Few {
     static constexpr int A = 128 * MM_TILE_K, STAGE = A + T * MM_TILE_K;
-    static constexpr int STAGES = T <= 32 ? 5 : T == 64 ? 4 : 3;   // two CTAs on an SM
-    static constexpr int BUFS = 2;
-    static constexpr uint32_t TMEM = BUFS * T < 32 ? 32 : BUFS * T;
-    static constexpr int SCALES = 4 * 2 * T * 4;                    // per warp: two sets of T factors
-    static constexpr int SMEM = STAGES * STAGE + SCALES + 256 + 1024;
+    static constexpr int PER_SM = T <= 64 ? 2 : 1;                  // CTAs on an SM
+    static constexpr int STAGES = T <= 32 ? 5 : T == 64 ? 4 : 6;
+    static constexpr int BUFS = T <= 64 ? 4 : 2;
+    static constexpr uint32_t TMEM = BUFS * T;                      // 64 to 256 columns
+    static constexpr int WARPS = T <= 64 ? 4 : 8;                   // warps that hold sums, each of 32 columns x ROWS rows
+    static constexpr int ROWS = 4 * T / WARPS;
+    static constexpr int THREADS = 32 * WARPS + 96;                 // then a warp each for copies, products, scales
+    static constexpr int SLOTS = 8, SLOT = 4 * (T + 4);             // blocks of scales in flight: T of x, one of w
+    static constexpr int SCALES = STAGES * STAGE, BARS = SCALES + SLOTS * SLOT, SMEM = BARS + 512 + 1024;
+    static_assert(8 * (2 * STAGES + 2 * BUFS + 2 * SLOTS + 1) + 4 <= 512, "room for the barriers");
+    static_assert(PER_SM * (SMEM + 1024) <= 228 * 1024, "more shared memory than an SM has");
     static_assert(STAGES * STAGE >= T * 128 * 4, "the sums are handed over in the stages' memory");
 };
-constexpr int MMF_THREADS = 192;  // warps 0-3 sums, 4 copies, 5 products
 
-template <typename OUT, int T> __global__ void __launch_bounds__(MMF_THREADS, 2) matmul_fp8_few_kernel(const __grid_constant__ MatmulParams p, int S) {
+template <typename OUT, int T>
+__global__ void __launch_bounds__(Few<T>::THREADS, Few<T>::PER_SM) matmul_fp8_few_kernel(const __grid_constant__ MatmulParams p, int S) {
     using C = Few<T>;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    const uint32_t base = smem_u32(smem);
-    const uint32_t bars = base + C::STAGES * C::STAGE + C::SCALES;
-    const uint32_t full = bars, empty = full + 8 * C::STAGES, done = empty + 8 * C::STAGES, taken = done + 8 * C::BUFS,
-                   last = taken + 8 * C::BUFS;
+    const uint32_t base = smem_u32(smem), full = base + C::BARS;
+    const uint32_t empty = full + 8 * C::STAGES, done = empty + 8 * C::STAGES, taken = done + 8 * C::BUFS,
+                   scaled = taken + 8 * C::BUFS, used = scaled + 8 * C::SLOTS, last = used + 8 * C::SLOTS;
     volatile uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + (last + 8 - base));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int b = 0; b < C::BUFS; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, 4); }
+        for (int b = 0; b < C::BUFS; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, C::WARPS); }
+        for (int f = 0; f < C::SLOTS; ++f) { mbar_init(scaled + 8 * f, 32); mbar_init(used + 8 * f, C::WARPS); }
         mbar_init(last, 1);
         fence_barrier_init();
     }
-    if (warp == 5) tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_at)), C::TMEM);
+    if (warp == C::WARPS + 1) tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_at)), C::TMEM);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
     const int rank = S > 1 ? (int)cluster_rank() : 0;
     const int n0 = ((int)blockIdx.x / S) * 128, m0 = (int)blockIdx.y * T;
-    const int kb0 = (int)((long long)p.n_kb * rank / S), kb1 = (int)((long long)p.n_kb * (rank + 1) / S);
-    const int n = n0 + (warp & 3) * 32 + lane;
-    float2 acc[T / 2];
+    const int kb0 = (int)((long long)p.n_kb * rank / S), blocks = (int)((long long)p.n_kb * (rank + 1) / S) - kb0;
+    const int n = n0 + (warp & 3) * 32 + lane, row0 = (warp >> 2) * C::ROWS;  // of the warps with sums
+    float2 acc[C::ROWS / 2];
+    bool ok = true;
 
-    if (warp == 4) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t s = it % C::STAGES, round = it / C::STAGES;
-                if (round > 0 && !mbar_wait_limit(empty + 8 * s, (round - 1) & 1)) { ok = false; break; }
+    if (warp == C::WARPS) {
+        for (int it = 0; it < blocks; ++it) {
+            const int s = it % C::STAGES, round = it / C::STAGES;
+            if (round > 0) ok = mbar_wait_limit(empty + 8 * s, (round - 1) & 1);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            if (elect_one()) {
                 mbar_expect_tx(full + 8 * s, C::STAGE);
-                tma_load_2d(base + s * C::STAGE, &p.w_map, full + 8 * s, kb * MM_TILE_K, n0);
-                tma_load_2d(base + s * C::STAGE + C::A, &p.x_map, full + 8 * s, kb * MM_TILE_K, m0);
+                tma_load_2d(base + s * C::STAGE, &p.w_map, full + 8 * s, (kb0 + it) * MM_TILE_K, n0);
+                tma_load_2d(base + s * C::STAGE + C::A, &p.x_map, full + 8 * s, (kb0 + it) * MM_TILE_K, m0);
             }
-            const uint32_t left = it < (uint32_t)C::STAGES ? it : (uint32_t)C::STAGES;
-            for (uint32_t i = it - left; i < it; ++i) ok &= mbar_wait_limit(full + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
-            if (!ok && p.status != nullptr) *p.status = MM_TIMEOUT;
         }
-    } else if (warp == 5) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = fp8_idesc(128, T);
-            uint32_t it = 0;
-            bool ok = true;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t s = it % C::STAGES, b = it % C::BUFS;
-                if (it >= (uint32_t)C::BUFS && !mbar_wait_limit(taken + 8 * b, (it / C::BUFS - 1) & 1)) { ok = false; break; }
-                if (!mbar_wait_limit(full + 8 * s, (it / C::STAGES) & 1)) { ok = false; break; }
-                tc_fence_after();
-                const uint64_t w = smem_operand(base + s * C::STAGE), x = smem_operand(base + s * C::STAGE + C::A);
+        // no copy outlives the CTA: the last rounds' products are done, or time is given
+        for (int i = blocks < C::STAGES ? 0 : blocks - C::STAGES; ok && i < blocks; ++i)
+            ok = mbar_wait_limit(empty + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
+        if (!ok) wait_ns(1000000);
+    } else if (warp == C::WARPS + 1) {
+        constexpr uint32_t idesc = fp8_idesc(128, T);
+        for (int it = 0; it < blocks; ++it) {
+            const int s = it % C::STAGES, b = it % C::BUFS, round = it / C::BUFS;
+            const uint64_t w = smem_operand(base + s * C::STAGE), x = smem_operand(base + s * C::STAGE + C::A);
+            ok = mbar_wait_limit(full + 8 * s, (it / C::STAGES) & 1);
+            if (round > 0) ok &= mbar_wait_limit(taken + 8 * b, (round - 1) & 1);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tc_mma_fp8(tmem + b * T, w + 2 * k, x + 2 * k, idesc, k > 0);
-                tc_commit(empty + 8 * s);
                 tc_commit(done + 8 * b);
+                tc_commit(empty + 8 * s);
             }
-            tc_commit(last);
-            ok &= mbar_wait_limit(last, 0);
-            if (!ok && p.status != nullptr) *p.status = MM_TIMEOUT;
+            __syncwarp();
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < T / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-        const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16);
-        constexpr int PER = (T + 31) / 32;  // rows whose factor a lane prepares
-        float* factors = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE) + warp * 2 * T;
-        const float* ws = p.w_scales + (long long)(n0 / 128) * p.ws_row;
+        if (elect_one()) tc_commit(last);  // no product outlives the CTA
+        ok &= mbar_wait_limit(last, 0);
+    } else if (warp == C::WARPS + 2) {
+        constexpr int PER = (T + 31) / 32;
+        const float* ws = p.w_scales + (long long)(n0 / 128) * p.ws_row + kb0 * p.ws_blk;
         const float* xs[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int m = m0 + i * 32 + lane;
-            xs[i] = p.x_scales + (long long)(m < p.M ? m : 0) * p.xs_row;
+            xs[i] = p.x_scales + (long long)(m < p.M ? m : 0) * p.xs_row + kb0 * p.xs_blk;
         }
-        float next[PER], wnext = 0.f;
+        for (int it = 0; it < blocks; ++it) {
+            const int f = it % C::SLOTS, round = it / C::SLOTS;
+            if (round > 0) ok = mbar_wait_limit(used + 8 * f, (round - 1) & 1);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            const uint32_t at = base + C::SCALES + f * C::SLOT;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) next[i] = 0.f;
-        if (kb0 < kb1) {
-            wnext = ws[kb0 * p.ws_blk];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) next[i] = xs[i][kb0 * p.xs_blk];
-        }
-        uint32_t it = 0;
-        bool ok = true;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            float* f = factors + (it & 1) * T;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (i * 32 + lane < T) f[i * 32 + lane] = next[i] * wnext;
-            __syncwarp();
-            if (kb + 1 < kb1) {
-                wnext = ws[(kb + 1) * p.ws_blk];
-#pragma unroll
-                for (int i = 0; i < PER; ++i) next[i] = xs[i][(kb + 1) * p.xs_blk];
+            for (int i = 0; i < PER; ++i) {
+                if (i * 32 + lane < T) copy_4(at + (i * 32 + lane) * 4, xs[i]);
+                xs[i] += p.xs_blk;
             }
-            const uint32_t b = it % C::BUFS;
-            if (!mbar_wait_limit(done + 8 * b, (it / C::BUFS) & 1)) { ok = false; break; }
+            if (lane == 0) copy_4(at + T * 4, ws);
+            ws += p.ws_blk;
+            copies_arrive(scaled + 8 * f);
+        }
+        copies_wait();
+    } else {
+#pragma unroll
+        for (int j = 0; j < C::ROWS / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+        const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + row0;
+        for (int it = 0; ok && it < blocks; ++it) {
+            const int f = it % C::SLOTS, b = it % C::BUFS;
+            const float* scale = reinterpret_cast<const float*>(smem + C::SCALES + f * C::SLOT);
+            ok = mbar_wait_limit(scaled + 8 * f, (it / C::SLOTS) & 1);
+            const float sw = scale[T];
+            ok &= mbar_wait_limit(done + 8 * b, (it / C::BUFS) & 1);
             tc_fence_after();
-            uint32_t r[2][16];
-            tmem_ld<16>(at + b * T, r[0]);
+            constexpr int L = C::ROWS < 32 ? C::ROWS : 32;  // rows read back at a time
 #pragma unroll
-            for (int c = 0; c < T / 16; ++c) {
-                tc_wait_ld(r[c & 1]);
-                if (c + 1 < T / 16) tmem_ld<16>(at + b * T + 16 * (c + 1), r[(c + 1) & 1]);
-                else {
+            for (int c = 0; c < C::ROWS / L; ++c) {
+                uint32_t r[L];
+                tmem_ld<L>(at + b * T + c * L, r);
+                tc_wait_ld(r);
+                if (c + 1 == C::ROWS / L) {
                     tc_fence_before();
-                    if (lane == 0) mbar_arrive(taken + 8 * b);
+                    __syncwarp();
+                    if (lane == 0 && ok) mbar_arrive(taken + 8 * b);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float4 s = *reinterpret_cast<const float4*>(f + 16 * c + 4 * j);
-                    fma_pair(acc[8 * c + 2 * j], as_pair(r[c & 1][4 * j], r[c & 1][4 * j + 1]), make_float2(s.x, s.y));
-                    fma_pair(acc[8 * c + 2 * j + 1], as_pair(r[c & 1][4 * j + 2], r[c & 1][4 * j + 3]), make_float2(s.z, s.w));
+                for (int j = 0; j < L / 4; ++j) {
+                    const float4 s = *reinterpret_cast<const float4*>(scale + row0 + c * L + 4 * j);
+                    fma_pair(acc[c * L / 2 + 2 * j], as_pair(r[4 * j], r[4 * j + 1]), make_float2(s.x * sw, s.y * sw));
+                    fma_pair(acc[c * L / 2 + 2 * j + 1], as_pair(r[4 * j + 2], r[4 * j + 3]), make_float2(s.z * sw, s.w * sw));
                 }
             }
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive(used + 8 * f);
         }
-        if (!ok && lane == 0 && p.status != nullptr) *p.status = MM_TIMEOUT;
     }
+    if (!ok && lane == 0 && p.status != nullptr) *p.status = MM_TIMEOUT;
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 5) tmem_free<1>(tmem, C::TMEM);
+    if (warp == C::WARPS + 1) tmem_free<1>(tmem, C::TMEM);
     if (S > 1) {
         float* sums = reinterpret_cast<float*>(smem);  // [T][128]
-        if (warp < 4) {
+        if (warp < C::WARPS) {
 #pragma unroll
-            for (int j = 0; j < T / 2; ++j) {
-                sums[(2 * j) * 128 + warp * 32 + lane] = acc[j].x;
-                sums[(2 * j + 1) * 128 + warp * 32 + lane] = acc[j].y;
+            for (int j = 0; j < C::ROWS / 2; ++j) {
+                sums[(row0 + 2 * j) * 128 + (warp & 3) * 32 + lane] = acc[j].x;
+                sums[(row0 + 2 * j + 1) * 128 + (warp & 3) * 32 + lane] = acc[j].y;
             }
         }
         cluster_sync();
-        if (warp < 4 && n < p.N) {
+        if (warp < C::WARPS && n < p.N) {
             const float bias = load_bias(p, n);
-            for (int j = rank; j < T && m0 + j < p.M; j += S) {
+            for (int j = rank + (warp >> 2) * S; j < T && m0 + j < p.M; j += S * (C::WARPS / 4)) {
                 float v = bias;
-                for (int q = 0; q < S; ++q) v += ld_cluster(base + (uint32_t)(j * 128 + warp * 32 + lane) * 4u, q);
+                for (int q = 0; q < S; ++q) v += ld_cluster(base + (uint32_t)(j * 128 + (warp & 3) * 32 + lane) * 4u, q);
                 static_cast<OUT*>(p.y)[(long long)(m0 + j) * p.y_stride + n] = from_f32<OUT>(v);
             }
         }
-        cluster_sync();
-    } else if (warp < 4 && n < p.N) {
+        cluster_sync();  // no CTA leaves while its sums may be read
+    } else if (warp < C::WARPS && n < p.N) {
         const float bias = load_bias(p, n);
-        OUT* y = static_cast<OUT*>(p.y) + (long long)m0 * p.y_stride + n;
+        OUT* y = static_cast<OUT*>(p.y) + (long long)(m0 + row0) * p.y_stride + n;
 #pragma unroll
-        for (int j = 0; j < T; ++j)
-            if (m0 + j < p.M) y[j * p.y_stride] = from_f32<OUT>(bias + (j & 1 ? acc[j / 2].y : acc[j / 2].x));
+        for (int j = 0; j < C::ROWS; ++j)
+            if (m0 + row0 + j < p.M) y[j * p.y_stride] = from_f32<OUT>(bias + (j & 1 ? acc[j / 2].y : acc[j / 2].x));
     }
 }
 
