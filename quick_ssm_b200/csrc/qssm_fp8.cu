@@ -80,15 +80,32 @@ struct MatmulPlan {
     int x_box, w_box;
 };
 
-MatmulPlan plan_matmul(long long M, long long N, int n_kb) {
-    const long long sms = sm_count();
+// Which kernel, and over how many CTAs a tile's k is cut: the shortest of these estimates in microseconds, fitted on a
+// B200 with CUDA graphs of 20 calls (N x K 1024x4096, 20480x1024, 4096x4096, 300x16384, 16384x512, 2500x1100, M 1 to
+// 4096).  Both sides there, many-rows / few-rows kernel: 64x1024x4096 19.5 / 8.3, 128x20480x1024 13.9 / 17.8,
+// 64x20480x1024 13.5 / 10.5, 1024x4096x4096 21.8 / 41.5, 512x300x16384 66.3 / 15.5.
+//   many rows: 0.47 per block of k and round of tiles over the pairs of SMs, 0.9 to end a round (2 more where rows of y
+//              are not on 16-byte boundaries), 3 to begin;
+//   few rows:  0.35 to 0.65 per block of k, 1 per round, 4 to begin, 0.6 to join k.  Clusters of 2, 4 and 8 CTAs are
+//              resident on about 148, 136 and 112 SMs (a cluster has to fit into one group of SMs).
+MatmulPlan plan_matmul(long long M, long long N, int n_kb, bool y_vec) {
+    const long long sms = sm_count(), pairs = sms / 2;
     const long long big = ((M + MMR_M - 1) / MMR_M) * ((N + MMR_N - 1) / MMR_N);
-    if (M > 64 && big >= sms / 2) return {0, 1, 128, 64};
+    double best = 3.0 + (double)((big + pairs - 1) / pairs) * (0.47 * n_kb + (y_vec ? 0.9 : 2.9));
+    MatmulPlan plan{0, 1, 128, 64};
     const int T = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const double per_block = T == 16 ? 0.35 : T == 32 ? 0.4 : T == 64 ? 0.5 : 0.65;
     const long long tiles = ((N + 127) / 128) * ((M + T - 1) / T);
-    int S = 1;
-    while (S < 8 && tiles * S * 2 <= 2 * sms && n_kb >= 4 * S) S *= 2;
-    return {T, S, T, 128};
+    for (int S = 1; S <= 8 && S <= n_kb; S *= 2) {
+        const long long seats = (T <= 64 ? 2 : 1) * (S == 8 ? sms * 3 / 4 : S == 4 ? sms * 11 / 12 : sms);
+        const double cost = 4.0 + (double)((tiles * S + seats - 1) / seats) * (per_block * ((n_kb + S - 1) / S) + 1.0) +
+                            (S > 1 ? 0.6 : 0.0);
+        if (cost < best) {
+            best = cost;
+            plan = MatmulPlan{T, S, T, 128};
+        }
+    }
+    return plan;
 }
 
 template <typename OUT, int T> int launch_few(const MatmulParams& p, int S, cudaStream_t stream) {
@@ -96,7 +113,7 @@ template <typename OUT, int T> int launch_few(const MatmulParams& p, int S, cuda
     const int rc = ensure_smem(kernel, Few<T>::SMEM);
     if (rc) return rc;
     const long long gx = (long long)((p.N + 127) / 128) * S, gy = (p.M + T - 1) / T;
-    if (gy > 65535 || gx >= (1ll << 31)) return QSSM_E_SHAPE;
+    if (gx >= (1ll << 31) || gy > 65535) return QSSM_E_SHAPE;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)gx, (unsigned)gy);
@@ -172,7 +189,7 @@ int qssm_matmul_fp8(const void* x, const float* x_scales, const void* w, const f
     p.bias_dtype = bias_dtype; p.status = status_word;
     const int es = dtype_size(out_dtype);
     p.y_vec = fits(y, y_stride, 16, es);
-    const MatmulPlan plan = plan_matmul(M, N, p.n_kb);
+    const MatmulPlan plan = plan_matmul(M, N, p.n_kb, p.y_vec);
     int rc;
     if ((rc = matrix_map(p.x_map, x, M, K, x_stride, -1, plan.x_box)) ||
         (rc = matrix_map(p.w_map, w, N, K, w_stride, -1, plan.w_box)))

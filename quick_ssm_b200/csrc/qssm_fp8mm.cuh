@@ -260,12 +260,14 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                 } else {  // rows of y on any boundary: each row's piece by consecutive lanes
                     __syncwarp();
                     const int rows = p.M - m0 < 32 ? p.M - m0 : 32, cols = p.N - n0 - c * COLS;
-                    for (int r = 0; r < rows; ++r) {
-                        T* dst = static_cast<T*>(p.y) + (long long)(m0 + r) * p.y_stride + n0 + c * COLS;
+                    T* dst = static_cast<T*>(p.y) + (long long)m0 * p.y_stride + n0 + c * COLS;
+#pragma unroll 8
+                    for (int r = 0; r < 32; ++r) {
 #pragma unroll
-                        for (int i = lane; i < COLS; i += 32)
-                            if (i < cols)
-                                dst[i] = *reinterpret_cast<const T*>(buf + r * 128 + (((i / V) ^ (r & 7)) << 4) + (i % V) * sizeof(T));
+                        for (int i = lane; i < COLS; i += 32) {
+                            const T v = *reinterpret_cast<const T*>(buf + r * 128 + (((i / V) ^ (r & 7)) << 4) + (i % V) * sizeof(T));
+                            if (r < rows && i < cols) dst[r * p.y_stride + i] = v;
+                        }
                     }
                 }
             }
@@ -441,10 +443,25 @@ __global__ void __launch_bounds__(Few<T>::THREADS, Few<T>::PER_SM) matmul_fp8_fe
         cluster_sync();
         if (warp < C::WARPS && n < p.N) {
             const float bias = load_bias(p, n);
-            for (int j = rank + (warp >> 2) * S; j < T && m0 + j < p.M; j += S * (C::WARPS / 4)) {
-                float v = bias;
-                for (int q = 0; q < S; ++q) v += ld_cluster(base + (uint32_t)(j * 128 + (warp & 3) * 32 + lane) * 4u, q);
-                static_cast<OUT*>(p.y)[(long long)(m0 + j) * p.y_stride + n] = from_f32<OUT>(v);
+            // four rows' partial sums on their way at once: a load from another SM takes longer than anything here
+            const int step = S * (C::WARPS / 4), rows = p.M - m0 < T ? p.M - m0 : T;
+            for (int j0 = rank + (warp >> 2) * S; j0 < rows; j0 += 4 * step) {
+                float v[4][8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const int j = j0 + i * step;
+                        v[i][q] = q < S && j < rows ? ld_cluster(base + (uint32_t)(j * 128 + (warp & 3) * 32 + lane) * 4u, q) : 0.f;
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + i * step;
+                    float sum = bias;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) sum += v[i][q];
+                    if (j < rows) static_cast<OUT*>(p.y)[(long long)(m0 + j) * p.y_stride + n] = from_f32<OUT>(sum);
+                }
             }
         }
         cluster_sync();  // no CTA leaves while its sums may be read
