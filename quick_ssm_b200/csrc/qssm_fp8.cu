@@ -84,14 +84,14 @@ struct MatmulPlan {
 // B200 with CUDA graphs of 20 calls (N x K 1024x4096, 20480x1024, 4096x4096, 300x16384, 16384x512, 2500x1100, M 1 to
 // 4096).  Both sides there, many-rows / few-rows kernel: 64x1024x4096 19.5 / 8.3, 128x20480x1024 13.9 / 17.8,
 // 64x20480x1024 13.5 / 10.5, 1024x4096x4096 21.8 / 41.5, 512x300x16384 66.3 / 15.5.
-//   many rows: 0.47 per block of k and round of tiles over the pairs of SMs, 0.9 to end a round (2 more where rows of y
-//              are not on 16-byte boundaries), 3 to begin;
+//   many rows: 0.47 per block of k and round of tiles over the pairs of SMs, 0.9 to end a round (0.7, 1.9, 5.6 more where
+//              the rows of y take words of 8, 4, 2 bytes only), 3 to begin;
 //   few rows:  0.35 to 0.65 per block of k, 1 per round, 4 to begin, 0.6 to join k.  Clusters of 2, 4 and 8 CTAs are
 //              resident on about 148, 136 and 112 SMs (a cluster has to fit into one group of SMs).
-MatmulPlan plan_matmul(long long M, long long N, int n_kb, bool y_vec) {
+MatmulPlan plan_matmul(long long M, long long N, int n_kb, double ragged_us) {
     const long long sms = sm_count(), pairs = sms / 2;
     const long long big = ((M + MMR_M - 1) / MMR_M) * ((N + MMR_N - 1) / MMR_N);
-    double best = 3.0 + (double)((big + pairs - 1) / pairs) * (0.47 * n_kb + (y_vec ? 0.9 : 2.9));
+    double best = 3.0 + (double)((big + pairs - 1) / pairs) * (0.47 * n_kb + 0.9 + ragged_us);
     MatmulPlan plan{0, 1, 128, 64};
     const int T = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const double per_block = T == 16 ? 0.35 : T == 32 ? 0.4 : T == 64 ? 0.5 : 0.65;
@@ -189,7 +189,8 @@ int qssm_matmul_fp8(const void* x, const float* x_scales, const void* w, const f
     p.bias_dtype = bias_dtype; p.status = status_word;
     const int es = dtype_size(out_dtype);
     p.y_vec = fits(y, y_stride, 16, es);
-    const MatmulPlan plan = plan_matmul(M, N, p.n_kb, p.y_vec);
+    p.y_word = fits(y, y_stride, 8, es) && N * es % 8 == 0 ? 8 : fits(y, y_stride, 4, es) && N * es % 4 == 0 ? 4 : 2;
+    const MatmulPlan plan = plan_matmul(M, N, p.n_kb, p.y_vec ? 0.0 : p.y_word == 8 ? 0.7 : p.y_word == 4 ? 1.9 : 5.6);
     int rc;
     if ((rc = matrix_map(p.x_map, x, M, K, x_stride, -1, plan.x_box)) ||
         (rc = matrix_map(p.w_map, w, N, K, w_stride, -1, plan.w_box)))

@@ -26,6 +26,7 @@ struct MatmulParams {
     int M, N, K, n_kb;      // n_kb: blocks of 128 along k
     int m_tiles, n_tiles;
     int bias_dtype, y_vec;  // y_vec: rows of y start on 16-byte boundaries
+    int y_word;             // the longest of 8, 4, 2 bytes that every row of y starts and ends on a multiple of
     int* status;
 };
 
@@ -66,6 +67,19 @@ constexpr int MMR_OUT = MMR_STAGES * MMR_STAGE, MMR_BIAS = MMR_OUT + MMR_WARPS *
 constexpr int MMR_REGS_SUMS = 216, MMR_REGS_HELP = 40;
 static_assert(256 * MMR_REGS_SUMS + 256 * MMR_REGS_HELP <= MMR_THREADS * 128, "more registers than the CTA has");
 static_assert(MMR_SMEM <= 227 * 1024, "more shared memory than a CTA has");
+
+// 32 rows of 128 bytes from shared memory (128-byte swizzle) to `dst`, W bytes a lane.
+template <int W>
+__device__ __forceinline__ void put_rows(const uint8_t* buf, uint8_t* dst, long long pitch, int rows, int bytes, int lane) {
+    constexpr int PER_ROW = 128 / W;  // lanes
+    using U = typename Word<W>::type;
+#pragma unroll 4
+    for (int i = lane; i < 32 * PER_ROW; i += 32) {
+        const int r = i / PER_ROW, at = (i % PER_ROW) * W;
+        const U v = *reinterpret_cast<const U*>(buf + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
+        if (r < rows && at < bytes) *reinterpret_cast<U*>(dst + r * pitch + at) = v;
+    }
+}
 
 template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MMR_THREADS, 1)
     matmul_fp8_rows_kernel(const __grid_constant__ MatmulParams p) {
@@ -257,18 +271,14 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                         if (n0 + c * COLS < p.N) tma_store_2d(&p.y_map, smem_u32(buf), n0 + c * COLS, m0);
                         tma_commit();
                     }
-                } else {  // rows of y on any boundary: each row's piece by consecutive lanes
+                } else {  // rows of y on any boundary: each row's 128 bytes by consecutive lanes, in the words that fit
                     __syncwarp();
-                    const int rows = p.M - m0 < 32 ? p.M - m0 : 32, cols = p.N - n0 - c * COLS;
-                    T* dst = static_cast<T*>(p.y) + (long long)m0 * p.y_stride + n0 + c * COLS;
-#pragma unroll 8
-                    for (int r = 0; r < 32; ++r) {
-#pragma unroll
-                        for (int i = lane; i < COLS; i += 32) {
-                            const T v = *reinterpret_cast<const T*>(buf + r * 128 + (((i / V) ^ (r & 7)) << 4) + (i % V) * sizeof(T));
-                            if (r < rows && i < cols) dst[r * p.y_stride + i] = v;
-                        }
-                    }
+                    const int rows = p.M - m0 < 32 ? p.M - m0 : 32, bytes = (p.N - n0 - c * COLS) * (int)sizeof(T);
+                    uint8_t* dst = static_cast<uint8_t*>(p.y) + ((long long)m0 * p.y_stride + n0 + c * COLS) * sizeof(T);
+                    const long long pitch = p.y_stride * sizeof(T);
+                    if (p.y_word == 8) put_rows<8>(buf, dst, pitch, rows, bytes, lane);
+                    else if (p.y_word == 4) put_rows<4>(buf, dst, pitch, rows, bytes, lane);
+                    else put_rows<2>(buf, dst, pitch, rows, bytes, lane);
                 }
             }
         }
