@@ -14,14 +14,23 @@
 // Columns are dealt to lanes in units: with V = 8 elements per access (16-bit data) a unit is 256 columns, lane l
 // owning columns 8l..8l+7; with V <= 4 it is 128 columns in 4/V accesses of V adjacent elements per lane.  Either way
 // a 128-column quantisation block lies in one access group of 16 or 32 lanes, and its largest magnitude is a shuffle
-// reduction.  V = 4 serves everything that has fp32 in it, V = 2 and 1 rows whose pitch or length allow no more.
+// reduction.  V = 4 serves what has fp32 in it and short rows of 16 bits, V = 2 and 1 rows whose pitch or length allow
+// no more.
+//
+// A row is held by 1, 2, 4 or 8 warps, 16 elements a lane (the backward keeps three values of each, packed as they came,
+// and the dw sums), which leaves room for 16 to 32 warps on an SM; a warp takes several rows of one unit at a time.
+// Measured on a B200 against the copy rate (6.54 TB/s), bf16 65536x1024: forward 88 us of 82, to e4m3 107 of 72,
+// backward 113 of 82 (32 elements a lane as floats, eight warps on an SM: 187); fp32 165 of 164, 140 of 133, 167 of 164.
 #pragma once
 #include "qssm_elem.cuh"
 
 namespace qssm {
 
 constexpr int ADDNORM_WARPS = 8;      // warps per CTA
-constexpr int ADDNORM_HELD = 32;      // elements of a row that a lane holds in registers
+
+
+
+constexpr int ADDNORM_HELD = 16;       // elements of a row that a lane holds in registers
 constexpr int ADDNORM_CTAS = 4;       // upper bound of CTAs per SM in the backward (sizes its scratch)
 
 struct AddNormParams {
@@ -80,7 +89,7 @@ __device__ __forceinline__ void load_weight(const AddNormParams& p, int unit, in
 #pragma unroll
     for (int a = 0; a < Unit<V>::ACC; ++a) {
         const int col = Unit<V>::col(unit, a, lane);
-        if constexpr (V >= 4) {
+        if constexpr (V >= 2) {
             if (p.w_vec) {
                 float t[V];
                 if (col < p.H) load_elems<float, V>(static_cast<const float*>(p.w) + col, t);
@@ -101,22 +110,24 @@ __device__ __forceinline__ void load_weight(const AddNormParams& p, int unit, in
         }
     }
 }
-// The sum over the row: one warp's, or the eight warps' partial sums added in warp order.  `red` alternates between
-// two sets of eight, so that one barrier per sum is enough.
+// The sum over the row of WPR warps, in warp order.  `red` alternates between two sets, so that one barrier per sum is
+// enough; rows of fewer warps than the CTA's have barriers of their own.
 template <int WPR> __device__ __forceinline__ float sum_row(float v, float (*red)[ADDNORM_WARPS], int& turn) {
     v = sum_warp(v);
     if constexpr (WPR > 1) {
-        if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = v;
-        __syncthreads();
+        const int warp = threadIdx.x >> 5, group = warp / WPR;
+        if ((threadIdx.x & 31) == 0) red[turn][warp] = v;
+        if constexpr (WPR == ADDNORM_WARPS) __syncthreads();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WPR) : "memory");
         v = 0.f;
 #pragma unroll
-        for (int k = 0; k < ADDNORM_WARPS; ++k) v += red[turn][k];
+        for (int k = 0; k < WPR; ++k) v += red[turn][group * WPR + k];
         turn ^= 1;
     }
     return v;
 }
 
-// One unit of y, 16/32 bits, or quantised: the lanes of a 128-column block agree on its largest magnitude.
+// One unit of y, 16/32 bits, or quantised (then -y is given): the lanes of a block agree on its largest magnitude.
 template <typename TX, int V, bool FP8, int EPT>
 __device__ __forceinline__ void put_unit(const AddNormParams& p, long long row, int unit, int lane, const float (&y)[EPT]) {
     if constexpr (!FP8) {
@@ -127,6 +138,7 @@ __device__ __forceinline__ void put_unit(const AddNormParams& p, long long row, 
         for (int i = 0; i < EPT; ++i) amax = max_nan(amax, fabsf(y[i]));
         amax = max_lanes<V == 8 ? 16 : 32>(amax);
         const float scale = fp8_scale(amax);
+        const Fp8Scale by(scale);
         uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.y_stride;
 #pragma unroll
         for (int a = 0; a < Unit<V>::ACC; ++a) {
@@ -134,7 +146,7 @@ __device__ __forceinline__ void put_unit(const AddNormParams& p, long long row, 
             float t[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) t[i] = y[a * V + i];
-            if (col < p.H) store_fp8<V>(q + col, t, scale);
+            if (col < p.H) store_fp8<V>(q + col, t, by);
         }
         const int first = Unit<V>::col(unit, 0, lane);
         if ((lane & (V == 8 ? 15 : 31)) == 0 && first < p.H)
@@ -142,16 +154,17 @@ __device__ __forceinline__ void put_unit(const AddNormParams& p, long long row, 
     }
 }
 
-// WPR: warps per row (1 or 8).  NU: units of a row held in registers by each of its warps, 0 for longer rows.
-template <typename TX, typename TR, int V, int WPR, int NU, bool FP8>
+// WPR: warps per row.  NU: units of a row held in registers by each of its warps, 0 for rows that are longer.  R: rows at
+// a time.
+template <typename TX, typename TR, int V, int WPR, int NU, int R, bool FP8>
 __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const AddNormParams p) {
     constexpr int EPT = Unit<V>::EPT, N = NU > 0 ? NU : 1;
+    static_assert(R == 1 || WPR == 1, "several rows at a time are a warp's own");
     __shared__ float red[2][ADDNORM_WARPS];
     int turn = 0;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int wid = WPR > 1 ? warp : 0;
-    const long long first = WPR > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * ADDNORM_WARPS + warp;
-    const long long step = WPR > 1 ? (long long)gridDim.x : (long long)gridDim.x * ADDNORM_WARPS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wid = warp % WPR;
+    constexpr int ROWS = ADDNORM_WARPS / WPR;  // row groups of a CTA
+    const long long step = (long long)gridDim.x * ROWS * R;
     const int H = p.H;
     const float inv_h = 1.f / (float)H;
     float w[N][EPT];
@@ -159,41 +172,62 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
 #pragma unroll
         for (int u = 0; u < N; ++u) load_weight<V>(p, u * WPR + wid, lane, w[u]);
     }
-    for (long long row = first; row < p.rows; row += step) {
-        const TX* xr = static_cast<const TX*>(p.x) + row * p.x_stride;
-        const TR* rr = static_cast<const TR*>(p.res) + row * p.res_stride;
-        TR* hr = static_cast<TR*>(p.h) + row * p.h_stride;
-        float ss = 0.f;
+    for (long long row0 = ((long long)blockIdx.x * ROWS + warp / WPR) * R; row0 < p.rows; row0 += step) {
         if constexpr (NU > 0) {
-            float h[N][EPT];
+            float h[R][N][EPT];
 #pragma unroll
-            for (int u = 0; u < N; ++u) load_unit<TX, V>(xr, u * WPR + wid, lane, H, h[u]);
+            for (int k = 0; k < R; ++k) {
+                const TX* xr = static_cast<const TX*>(p.x) + (row0 + k) * p.x_stride;
+                const int cols = R == 1 || row0 + k < p.rows ? H : 0;
+#pragma unroll
+                for (int u = 0; u < N; ++u) load_unit<TX, V>(xr, u * WPR + wid, lane, cols, h[k][u]);
+            }
             if (p.res != nullptr) {
-                float t[N][EPT];
+                float t[R][N][EPT];
 #pragma unroll
-                for (int u = 0; u < N; ++u) load_unit<TR, V>(rr, u * WPR + wid, lane, H, t[u]);
+                for (int k = 0; k < R; ++k) {
+                    const TR* rr = static_cast<const TR*>(p.res) + (row0 + k) * p.res_stride;
+                    const int cols = R == 1 || row0 + k < p.rows ? H : 0;
 #pragma unroll
-                for (int u = 0; u < N; ++u) {
+                    for (int u = 0; u < N; ++u) load_unit<TR, V>(rr, u * WPR + wid, lane, cols, t[k][u]);
+                }
 #pragma unroll
-                    for (int i = 0; i < EPT; ++i) h[u][i] = to_f32(from_f32<TR>(h[u][i] + t[u][i]));
-                    store_unit<TR, V>(hr, u * WPR + wid, lane, H, h[u]);
+                for (int k = 0; k < R; ++k) {
+                    TR* hr = static_cast<TR*>(p.h) + (row0 + k) * p.h_stride;
+                    const int cols = R == 1 || row0 + k < p.rows ? H : 0;
+#pragma unroll
+                    for (int u = 0; u < N; ++u) {
+#pragma unroll
+                        for (int i = 0; i < EPT; ++i) h[k][u][i] = to_f32(from_f32<TR>(h[k][u][i] + t[k][u][i]));
+                        store_unit<TR, V>(hr, u * WPR + wid, lane, cols, h[k][u]);
+                    }
                 }
             }
 #pragma unroll
-            for (int u = 0; u < N; ++u)
+            for (int k = 0; k < R; ++k) {
+                float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < EPT; ++i) ss = fmaf(h[u][i], h[u][i], ss);
-            ss = sum_row<WPR>(ss, red, turn);
-            const float r = 1.f / sqrtf(ss * inv_h + p.eps);
-            if (p.rstd != nullptr && lane == 0 && wid == 0) p.rstd[row] = r;
+                for (int u = 0; u < N; ++u)
 #pragma unroll
-            for (int u = 0; u < N; ++u) {
+                    for (int i = 0; i < EPT; ++i) ss = fmaf(h[k][u][i], h[k][u][i], ss);
+                ss = sum_row<WPR>(ss, red, turn);
+                if (R > 1 && row0 + k >= p.rows) break;
+                float r = 1.f / sqrtf(ss * inv_h + p.eps);
+                if (p.rstd != nullptr && lane == 0 && wid == 0) p.rstd[row0 + k] = r;
+                if constexpr (FP8) r = -r;
 #pragma unroll
-                for (int i = 0; i < EPT; ++i) h[u][i] *= w[u][i] * r;
-                put_unit<TX, V, FP8>(p, row, u * WPR + wid, lane, h[u]);
+                for (int u = 0; u < N; ++u) {
+#pragma unroll
+                    for (int i = 0; i < EPT; ++i) h[k][u][i] *= w[u][i] * r;
+                    put_unit<TX, V, FP8>(p, row0 + k, u * WPR + wid, lane, h[k][u]);
+                }
             }
         } else {
+            const TX* xr = static_cast<const TX*>(p.x) + row0 * p.x_stride;
+            const TR* rr = static_cast<const TR*>(p.res) + row0 * p.res_stride;
+            TR* hr = static_cast<TR*>(p.h) + row0 * p.h_stride;
             const int units = (H + Unit<V>::COLS - 1) / Unit<V>::COLS;
+            float ss = 0.f;
             for (int u = wid; u < units; u += WPR) {
                 float h[EPT];
                 load_unit<TX, V>(xr, u, lane, H, h);
@@ -208,8 +242,9 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
                 for (int i = 0; i < EPT; ++i) ss = fmaf(h[i], h[i], ss);
             }
             ss = sum_row<WPR>(ss, red, turn);
-            const float r = 1.f / sqrtf(ss * inv_h + p.eps);
-            if (p.rstd != nullptr && lane == 0 && wid == 0) p.rstd[row] = r;
+            float r = 1.f / sqrtf(ss * inv_h + p.eps);
+            if (p.rstd != nullptr && lane == 0 && wid == 0) p.rstd[row0] = r;
+            if constexpr (FP8) r = -r;
             for (int u = wid; u < units; u += WPR) {  // a lane reads back what it wrote itself
                 float h[EPT], wu[EPT];
                 if (p.res != nullptr) load_unit<TR, V>(hr, u, lane, H, h);
@@ -217,25 +252,43 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
                 load_weight<V>(p, u, lane, wu);
 #pragma unroll
                 for (int i = 0; i < EPT; ++i) h[i] *= wu[i] * r;
-                put_unit<TX, V, FP8>(p, row, u, lane, h);
+                put_unit<TX, V, FP8>(p, row0, u, lane, h);
             }
         }
     }
 }
 
+// A unit of a row as it lies in memory (16-bit elements two to a register).
+template <typename T, int V> struct Packed {
+    static constexpr int EPT = Unit<V>::EPT;
+    alignas(16) T e[EPT];
+    __device__ __forceinline__ void load(const T* row, int unit, int lane, int cols) {
+        constexpr int BYTES = V * (int)sizeof(T) > 16 ? 16 : V * (int)sizeof(T), WORDS = EPT * (int)sizeof(T) / BYTES,
+                      PER_ACC = WORDS / Unit<V>::ACC;
+        using W = typename Word<BYTES>::type;
+        W* w = reinterpret_cast<W*>(e);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            const int col = Unit<V>::col(unit, i / PER_ACC, lane) + (i % PER_ACC) * (BYTES / (int)sizeof(T));
+            w[i] = W{};
+            if (col < cols) w[i] = *reinterpret_cast<const W*>(row + col);
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return to_f32(e[i]); }
+};
+
 // Backward.  Each warp keeps the dw sums of its columns: in registers over all its rows (NU > 0), added up over the
-// CTA's warps in warp order at the end where every warp has rows of its own; for longer rows (eight warps each) in the
-// CTA's part of the scratch.
-template <typename TX, typename TR, int V, int WPR, int NU>
+// CTA's row groups in order at the end; for longer rows (eight warps each) in the CTA's part of the scratch.  What a row
+// brings stays packed as it came.
+template <typename TX, typename TR, int V, int WPR, int NU, int R>
 __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const AddNormParams p) {
     constexpr int EPT = Unit<V>::EPT, N = NU > 0 ? NU : 1;
     __shared__ float red[2][ADDNORM_WARPS];
-    extern __shared__ float dw_sum[];  // WPR == 1, NU > 0: H floats
+    extern __shared__ float dw_sum[];  // WPR < 8, NU > 0: H floats
     int turn = 0;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int wid = WPR > 1 ? warp : 0;
-    const long long first = WPR > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * ADDNORM_WARPS + warp;
-    const long long step = WPR > 1 ? (long long)gridDim.x : (long long)gridDim.x * ADDNORM_WARPS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wid = warp % WPR;
+    constexpr int ROWS = ADDNORM_WARPS / WPR;
+    const long long step = (long long)gridDim.x * ROWS * R;
     const int H = p.H;
     const int units = (H + Unit<V>::COLS - 1) / Unit<V>::COLS;
     const float inv_h = 1.f / (float)H;
@@ -248,50 +301,69 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
     if constexpr (NU == 0) {
         for (int u = wid; u < units; u += WPR) store_unit<float, V>(part, u, lane, H, dw[0]);
     }
-    for (long long row = first; row < p.rows; row += step) {
-        const TR* hr = static_cast<const TR*>(p.h) + row * p.h_stride;
-        const TX* gr = static_cast<const TX*>(p.dy) + row * p.dy_stride;
-        const TR* er = static_cast<const TR*>(p.dh) + row * p.dh_stride;
-        TX* dxr = static_cast<TX*>(p.dx) + row * p.dx_stride;
-        TR* drr = static_cast<TR*>(p.dres) + row * p.dres_stride;
-        const float r = p.rstd[row];
-        float dot = 0.f;
+    for (long long row0 = ((long long)blockIdx.x * ROWS + warp / WPR) * R; row0 < p.rows; row0 += step) {
         if constexpr (NU > 0) {
-            float h[N][EPT], g[N][EPT], e[N][EPT];
+            Packed<TR, V> h[R][N], e[R][N];
+            Packed<TX, V> g[R][N];
+            float r[R];
 #pragma unroll
-            for (int u = 0; u < N; ++u) {
-                load_unit<TR, V>(hr, u * WPR + wid, lane, H, h[u]);
-                load_unit<TX, V>(gr, u * WPR + wid, lane, H, g[u]);
-            }
+            for (int k = 0; k < R; ++k) {
+                const long long row = row0 + k;
+                const int cols = R == 1 || row < p.rows ? H : 0;
+                r[k] = cols > 0 ? p.rstd[row] : 0.f;
 #pragma unroll
-            for (int u = 0; u < N; ++u) {
-                if (p.dh != nullptr) load_unit<TR, V>(er, u * WPR + wid, lane, H, e[u]);
-                else {
-#pragma unroll
-                    for (int i = 0; i < EPT; ++i) e[u][i] = 0.f;
+                for (int u = 0; u < N; ++u) {
+                    h[k][u].load(static_cast<const TR*>(p.h) + row * p.h_stride, u * WPR + wid, lane, cols);
+                    g[k][u].load(static_cast<const TX*>(p.dy) + row * p.dy_stride, u * WPR + wid, lane, cols);
                 }
+                const int ecols = p.dh != nullptr ? cols : 0;
+#pragma unroll
+                for (int u = 0; u < N; ++u)
+                    e[k][u].load(static_cast<const TR*>(p.dh) + row * p.dh_stride, u * WPR + wid, lane, ecols);
             }
+            float dot[R];
+#pragma unroll
+            for (int k = 0; k < R; ++k) dot[k] = 0.f;
 #pragma unroll
             for (int u = 0; u < N; ++u) {
                 float w[EPT];
                 load_weight<V>(p, u * WPR + wid, lane, w);
 #pragma unroll
-                for (int i = 0; i < EPT; ++i) {
-                    dw[u][i] = fmaf(g[u][i] * r, h[u][i], dw[u][i]);
-                    g[u][i] *= w[i];
-                    dot = fmaf(h[u][i], g[u][i], dot);
-                }
+                for (int k = 0; k < R; ++k)
+#pragma unroll
+                    for (int i = 0; i < EPT; ++i) {
+                        dw[u][i] = fmaf(g[k][u][i] * r[k], h[k][u][i], dw[u][i]);
+                        dot[k] = fmaf(h[k][u][i], g[k][u][i] * w[i], dot[k]);
+                    }
             }
-            dot = sum_row<WPR>(dot, red, turn);
-            const float k = dot * inv_h * r * r * r;
+#pragma unroll
+            for (int k = 0; k < R; ++k) dot[k] = sum_row<WPR>(dot[k], red, turn) * inv_h * r[k] * r[k] * r[k];
 #pragma unroll
             for (int u = 0; u < N; ++u) {
+                float w[EPT];
+                load_weight<V>(p, u * WPR + wid, lane, w);
 #pragma unroll
-                for (int i = 0; i < EPT; ++i) e[u][i] += fmaf(-h[u][i], k, r * g[u][i]);
-                if (p.dx != nullptr) store_unit<TX, V>(dxr, u * WPR + wid, lane, H, e[u]);
-                if (p.dres != nullptr) store_unit<TR, V>(drr, u * WPR + wid, lane, H, e[u]);
+                for (int k = 0; k < R; ++k) {
+                    const long long row = row0 + k;
+                    const int cols = R == 1 || row < p.rows ? H : 0;
+                    float d[EPT];
+#pragma unroll
+                    for (int i = 0; i < EPT; ++i)
+                        d[i] = e[k][u][i] + fmaf(-h[k][u][i], dot[k], r[k] * (g[k][u][i] * w[i]));
+                    if (p.dx != nullptr)
+                        store_unit<TX, V>(static_cast<TX*>(p.dx) + row * p.dx_stride, u * WPR + wid, lane, cols, d);
+                    if (p.dres != nullptr)
+                        store_unit<TR, V>(static_cast<TR*>(p.dres) + row * p.dres_stride, u * WPR + wid, lane, cols, d);
+                }
             }
         } else {
+            const TR* hr = static_cast<const TR*>(p.h) + row0 * p.h_stride;
+            const TX* gr = static_cast<const TX*>(p.dy) + row0 * p.dy_stride;
+            const TR* er = static_cast<const TR*>(p.dh) + row0 * p.dh_stride;
+            TX* dxr = static_cast<TX*>(p.dx) + row0 * p.dx_stride;
+            TR* drr = static_cast<TR*>(p.dres) + row0 * p.dres_stride;
+            const float r = p.rstd[row0];
+            float dot = 0.f;
             for (int u = wid; u < units; u += WPR) {
                 float h[EPT], g[EPT], w[EPT], s[EPT];
                 load_unit<TR, V>(hr, u, lane, H, h);
@@ -322,21 +394,22 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
             }
         }
     }
-    if constexpr (NU > 0 && WPR > 1) {
+    if constexpr (NU > 0 && WPR == ADDNORM_WARPS) {
 #pragma unroll
         for (int u = 0; u < N; ++u) store_unit<float, V>(part, u * WPR + wid, lane, H, dw[u]);
     } else if constexpr (NU > 0) {
-        for (int k = 0; k < ADDNORM_WARPS; ++k) {
-            if (warp == k) {
+        __syncthreads();
+        for (int k = 0; k < ROWS; ++k) {
+            if (warp / WPR == k) {
 #pragma unroll
                 for (int u = 0; u < N; ++u) {
                     float s[EPT];
 #pragma unroll
                     for (int i = 0; i < EPT; ++i) s[i] = 0.f;
-                    if (k > 0) load_unit<float, V>(dw_sum, u, lane, H, s);
+                    if (k > 0) load_unit<float, V>(dw_sum, u * WPR + wid, lane, H, s);
 #pragma unroll
                     for (int i = 0; i < EPT; ++i) s[i] += dw[u][i];
-                    store_unit<float, V>(k + 1 < ADDNORM_WARPS ? dw_sum : part, u, lane, H, s);
+                    store_unit<float, V>(k + 1 < ROWS ? dw_sum : part, u * WPR + wid, lane, H, s);
                 }
             }
             __syncthreads();

@@ -41,24 +41,21 @@ int qssm_add_rmsnorm_bwd(const void* h, const void* w, const void* dy, const voi
     p.w_dtype = w_dtype;
     p.w_vec = w_dtype == QSSM_F32 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
     const int es = dtype_size(x_dtype), rs = dtype_size(res_dtype);
-    int V = es == 2 && rs == 2 ? 8 : 4;
-    for (; V > 1; V = V == 8 ? 2 : 1) {
-        if (H % V == 0 && addnorm_fits(h, h_stride, rs, V) && addnorm_fits(dy, dy_stride, es, V) &&
-            addnorm_fits(dh, dh_stride, rs, V) && addnorm_fits(dx, dx_stride, es, V) &&
-            addnorm_fits(dres, dres_stride, rs, V))
-            break;
-    }
+    const int V = addnorm_access(es, rs, H, [&](int v) {
+        return addnorm_fits(h, h_stride, rs, v) && addnorm_fits(dy, dy_stride, es, v) && addnorm_fits(dh, dh_stride, rs, v) &&
+               addnorm_fits(dx, dx_stride, es, v) && addnorm_fits(dres, dres_stride, rs, v);
+    });
     int n_part = 0;
     const int err = addnorm_types(x_dtype, res_dtype, [&](auto tx, auto tr) -> int {
         using TX = decltype(tx);
         using TR = decltype(tr);
-        return addnorm_variant<TX, TR>(V, rows, (int)H, [&](auto v, auto wpr, auto nu) -> int {
-            constexpr int W = decltype(wpr)::value, NU = decltype(nu)::value;
-            const long long need = W > 1 ? rows : (rows + ADDNORM_WARPS - 1) / ADDNORM_WARPS;
-            const long long most = (long long)ADDNORM_CTAS * sm_count();
+        return addnorm_variant<TX, TR>(V, rows, (int)H, [&](auto v, auto wpr, auto nu, auto at_once) -> int {
+            constexpr int W = decltype(wpr)::value, NU = decltype(nu)::value, R = decltype(at_once)::value,
+                          ROWS = ADDNORM_WARPS / W * R;
+            const long long need = (rows + ROWS - 1) / ROWS, most = (long long)ADDNORM_CTAS * sm_count();
             n_part = (int)(need < most ? need : most);
-            const int smem = W == 1 && NU > 0 ? (int)H * 4 : 0;  // at most 4 KB
-            addnorm_bwd_kernel<TX, TR, decltype(v)::value, W, NU><<<(unsigned)n_part, 32 * ADDNORM_WARPS, smem, stream>>>(p);
+            const int smem = W < ADDNORM_WARPS && NU > 0 ? (int)H * 4 : 0;  // at most 16 KB
+            addnorm_bwd_kernel<TX, TR, decltype(v)::value, W, NU, R><<<(unsigned)n_part, 32 * ADDNORM_WARPS, smem, stream>>>(p);
             return (int)cudaGetLastError();
         });
     });

@@ -10,20 +10,17 @@ namespace {
 template <bool FP8> int run_forward(AddNormParams& p, int x_dtype, int res_dtype, cudaStream_t stream) {
     const int es = dtype_size(x_dtype), rs = dtype_size(res_dtype);
     const bool has_res = p.res != nullptr;
-    int V = es == 2 && rs == 2 ? 8 : 4;
-    for (; V > 1; V = V == 8 ? 2 : 1) {
-        if (p.H % V == 0 && addnorm_fits(p.x, p.x_stride, es, V) && addnorm_fits(p.y, p.y_stride, FP8 ? 1 : es, V) &&
-            (!has_res || (addnorm_fits(p.res, p.res_stride, rs, V) && addnorm_fits(p.h, p.h_stride, rs, V))))
-            break;
-    }
+    const int V = addnorm_access(es, rs, p.H, [&](int v) {
+        return addnorm_fits(p.x, p.x_stride, es, v) && addnorm_fits(p.y, p.y_stride, FP8 ? 1 : es, v) &&
+               (!has_res || (addnorm_fits(p.res, p.res_stride, rs, v) && addnorm_fits(p.h, p.h_stride, rs, v)));
+    });
     return addnorm_types(x_dtype, res_dtype, [&](auto tx, auto tr) -> int {
         using TX = decltype(tx);
         using TR = decltype(tr);
-        return addnorm_variant<TX, TR>(V, p.rows, p.H, [&](auto v, auto wpr, auto nu) -> int {
-            constexpr int W = decltype(wpr)::value;
-            const long long need = W > 1 ? p.rows : (p.rows + ADDNORM_WARPS - 1) / ADDNORM_WARPS;
-            const long long most = 8ll * sm_count();
-            addnorm_fwd_kernel<TX, TR, decltype(v)::value, W, decltype(nu)::value, FP8>
+        return addnorm_variant<TX, TR>(V, p.rows, p.H, [&](auto v, auto wpr, auto nu, auto at_once) -> int {
+            constexpr int W = decltype(wpr)::value, R = decltype(at_once)::value, ROWS = ADDNORM_WARPS / W * R;
+            const long long need = (p.rows + ROWS - 1) / ROWS, most = 8ll * sm_count();
+            addnorm_fwd_kernel<TX, TR, decltype(v)::value, W, decltype(nu)::value, R, FP8>
                 <<<(unsigned)(need < most ? need : most), 32 * ADDNORM_WARPS, 0, stream>>>(p);
             return (int)cudaGetLastError();
         });

@@ -25,26 +25,37 @@ template <typename F> int addnorm_types(int x_dtype, int res_dtype, F&& f) {
     }
 }
 
-// Calls f(Int<V>, Int<WPR>, Int<NU>).  One warp per row for rows of up to 256 elements, and up to 1024 where there are
-// enough rows to fill the GPU with such warps (16 per SM); eight warps per row otherwise.
+// Elements per access for rows of H columns: the largest that `fits(V)` every tensor.  Short rows of 16-bit data take
+// units of 128 columns (V = 4): with 256 half of the lanes would have nothing.
+template <typename F> int addnorm_access(int es, int rs, long long H, F&& fits) {
+    for (int V = es == 2 && rs == 2 && H > 128 ? 8 : 4; V > 1; V /= 2)
+        if (H % V == 0 && fits(V)) return V;
+    return 1;
+}
+
+// Calls f(Int<V>, Int<WPR>, Int<NU>, Int<R>): as few warps per row as hold it, ADDNORM_HELD elements a lane (eight warps
+// with twice as many, then a second read, behind that); more warps per row where there are fewer rows than warps to fill
+// the GPU (16 per SM); several rows per warp at a time where a row is one unit.
 template <typename TX, typename TR, typename F> int addnorm_variant(int V, long long rows, int H, F&& f) {
-    const bool one_warp = H <= 256 || (H <= 32 * ADDNORM_HELD && rows >= 16ll * sm_count());
     auto go = [&](auto v) -> int {
-        constexpr int VV = decltype(v)::value;
-        constexpr int FULL = ADDNORM_HELD / Unit<VV>::EPT, QUARTER = FULL / 4;
+        constexpr int VV = decltype(v)::value, FULL = ADDNORM_HELD / Unit<VV>::EPT;
         const int units = (H + Unit<VV>::COLS - 1) / Unit<VV>::COLS;
-        const int held = one_warp ? units : (units + ADDNORM_WARPS - 1) / ADDNORM_WARPS;
-        if (one_warp) return held <= QUARTER ? f(v, AnInt<1>{}, AnInt<QUARTER>{}) : f(v, AnInt<1>{}, AnInt<FULL>{});
-        if (held <= QUARTER) return f(v, AnInt<ADDNORM_WARPS>{}, AnInt<QUARTER>{});
-        if (held <= FULL) return f(v, AnInt<ADDNORM_WARPS>{}, AnInt<FULL>{});
-        return f(v, AnInt<ADDNORM_WARPS>{}, AnInt<0>{});
+        const long long want = 16ll * sm_count();  // warps
+        if (units <= 1) return f(v, AnInt<1>{}, AnInt<1>{}, AnInt<FULL>{});
+        if (units <= FULL && rows >= want) return f(v, AnInt<1>{}, AnInt<FULL>{}, AnInt<1>{});
+        if constexpr (VV >= 4) {
+            if (units <= 2 * FULL && 2 * rows >= want) return f(v, AnInt<2>{}, AnInt<FULL>{}, AnInt<1>{});
+        }
+        if (units <= 4 * FULL && (VV < 4 || 4 * rows >= want)) return f(v, AnInt<4>{}, AnInt<FULL>{}, AnInt<1>{});
+        if (units <= 8 * FULL) return f(v, AnInt<8>{}, AnInt<FULL>{}, AnInt<1>{});
+        if (units <= 16 * FULL) return f(v, AnInt<8>{}, AnInt<2 * FULL>{}, AnInt<1>{});
+        return f(v, AnInt<8>{}, AnInt<0>{}, AnInt<1>{});
     };
     if constexpr (sizeof(TX) == 2 && sizeof(TR) == 2) {
         if (V == 8) return go(AnInt<8>{});
-        if (V == 2) return go(AnInt<2>{});
-    } else {
-        if (V == 4) return go(AnInt<4>{});
     }
+    if (V == 4) return go(AnInt<4>{});
+    if (V == 2) return go(AnInt<2>{});
     return go(AnInt<1>{});
 }
 

@@ -141,14 +141,17 @@ int qssm_quant_fp8_rows(const void* x, void* q, float* scales, int64_t rows, int
     QuantParams p{x, static_cast<uint8_t*>(q), scales, rows, x_stride, q_stride, scale_stride_row, scale_stride_blk, (int)K};
     return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        constexpr int V = 16 / sizeof(T), COLS = 32 * V;
-        const bool vec = K % V == 0 && fits(x, x_stride, 16, sizeof(T)) && fits(q, q_stride, V, 1);
-        const long long cols = vec ? COLS : FP8_BLOCK;
-        const long long units = (K + cols - 1) / cols, jobs = rows * ((units + QUANT_UNITS - 1) / QUANT_UNITS);
+        constexpr int VEC = 16 / sizeof(T);
+        int V = K > 128 ? VEC : 4;  // as many elements per access as every row allows; short rows in units of 128
+        while (V > 1 && !(K % V == 0 && fits(x, x_stride, V * (int)sizeof(T), sizeof(T)) && fits(q, q_stride, V, 1))) V /= 2;
+        const long long cols = V == 8 ? 256 : 128, jobs = (rows + QUANT_ROWS - 1) / QUANT_ROWS * ((K + cols - 1) / cols);
         const long long need = (jobs + 7) / 8, most = 16ll * sm_count();
         const unsigned grid = (unsigned)(need < most ? need : most);
-        if (vec) quant_rows_kernel<T, V><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-        else quant_rows_kernel<T, 1><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (V == VEC) quant_rows_kernel<T, VEC><<<grid, 256, 0, s>>>(p);
+        else if (V == 4) quant_rows_kernel<T, 4><<<grid, 256, 0, s>>>(p);
+        else if (V == 2) quant_rows_kernel<T, 2><<<grid, 256, 0, s>>>(p);
+        else quant_rows_kernel<T, 1><<<grid, 256, 0, s>>>(p);
         return (int)cudaGetLastError();
     });
 }

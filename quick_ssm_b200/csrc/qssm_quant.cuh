@@ -1,8 +1,8 @@
 // Quantisation to e4m3 with a scale for each 128 values of a row (activations) or each 128 x 128 block (weights).
 //
-// Bound by memory: one read of the source, one byte written per value.  Rows: a warp takes up to four adjacent units of a
-// row (a unit is 256 columns in 16-byte accesses for 16-bit data, 128 otherwise), all loads first, then a shuffle
-// reduction per 128-column block.  Weights: a CTA takes one block, each warp 16 of its rows, and keeps it in registers
+// Bound by memory: one read of the source, one byte written per value.  Rows: a warp takes one unit of
+// four adjacent rows at a time (a unit is 256 columns in 16-byte accesses for 16-bit data, 128 otherwise), whose scales
+// lie side by side, with the next four on their way; a reduction over lanes per 128-column block.  Weights: a CTA takes one block, each warp 16 of its rows, and keeps it in registers
 // between the reduction and the output.
 #pragma once
 #include "qssm_elem.cuh"
@@ -17,49 +17,96 @@ struct QuantParams {
     int K;
 };
 
-constexpr int QUANT_UNITS = 4;  // units a warp has in flight
+constexpr int QUANT_ROWS = 4;  // rows whose unit a warp takes at a time
+
+// One unit of a row as it lies in memory (16-bit elements two to a register), zeros outside.
+template <typename T, int V> struct QuantUnit {
+    static constexpr int EPT = V == 8 ? 8 : 4, COLS = 32 * EPT, ACC = EPT / V, BYTES = V * (int)sizeof(T);
+    using W = typename Word<BYTES>::type;
+    alignas(16) T e[EPT];
+    __device__ __forceinline__ void load(const T* row, int unit, int lane, int cols) {
+#pragma unroll
+        for (int a = 0; a < ACC; ++a) {
+            const int col = unit * COLS + a * 32 * V + lane * V;
+            W w{};
+            if (col < cols) w = *reinterpret_cast<const W*>(row + col);
+            reinterpret_cast<W*>(e)[a] = w;
+        }
+    }
+    // the largest magnitude, NaN if there is one; 16-bit types two at a time
+    __device__ __forceinline__ float amax() const {
+        if constexpr (std::is_same<T, float>::value) {
+            float m = fabsf(e[0]);
+#pragma unroll
+            for (int i = 1; i < EPT; ++i) m = max_nan(m, fabsf(e[i]));
+            return m;
+        } else {
+            using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            const T2* v = reinterpret_cast<const T2*>(e);
+            T2 m = __habs2(v[0]);
+#pragma unroll
+            for (int i = 1; i < EPT / 2; ++i) m = __hmax2_nan(m, __habs2(v[i]));
+            return max_nan(to_f32(m.x), to_f32(m.y));
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* row, int unit, int lane, int cols, const Fp8Scale& by) const {
+#pragma unroll
+        for (int a = 0; a < ACC; ++a) {
+            const int col = unit * COLS + a * 32 * V + lane * V;
+            alignas(16) T ne[V];  // negated, 16-bit types two at a time
+            if constexpr (sizeof(T) == 2 && V >= 2) {
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i)
+                    reinterpret_cast<uint32_t*>(ne)[i] = reinterpret_cast<const uint32_t*>(e + a * V)[i] ^ 0x80008000u;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) ne[i] = -e[a * V + i];
+            }
+            float t[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[i] = to_f32(ne[i]);
+            if (col < cols) store_fp8<V>(row + col, t, by);
+        }
+    }
+};
 
 template <typename T, int V> __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p) {
-    constexpr int EPT = V == 8 ? 8 : 4, COLS = 32 * EPT, ACC = EPT / V;
+    using U = QuantUnit<T, V>;
+    constexpr int N = QUANT_ROWS, HALF = V == 8 ? 16 : 32;  // lanes of a block
     const int lane = threadIdx.x & 31;
-    const int units = (p.K + COLS - 1) / COLS, groups = (units + QUANT_UNITS - 1) / QUANT_UNITS;
-    const long long jobs = p.rows * groups, step = (long long)gridDim.x * 8;
-    for (long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); job < jobs; job += step) {
-        const long long row = job / groups;
-        const int u0 = (int)(job - row * groups) * QUANT_UNITS;
-        const T* xr = static_cast<const T*>(p.x) + row * p.x_stride;
-        uint8_t* qr = p.q + row * p.q_stride;
-        float v[QUANT_UNITS][EPT];
+    const int units = (p.K + U::COLS - 1) / U::COLS;
+    const long long jobs = (p.rows + N - 1) / N * units, step = (long long)gridDim.x * 8;
+    long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (job >= jobs) return;
+    U now[N], next[N];
+    auto fetch = [&](U (&into)[N], long long row, int unit) {
 #pragma unroll
-        for (int u = 0; u < QUANT_UNITS; ++u)
+        for (int i = 0; i < N; ++i)
+            into[i].load(static_cast<const T*>(p.x) + (row + i) * p.x_stride, unit, lane, row + i < p.rows ? p.K : 0);
+    };
+    long long row = job / units * N;
+    int unit = (int)(job % units);
+    fetch(now, row, unit);
+    for (;;) {  // the next units are on their way while these are worked on
+        job += step;
+        const long long row1 = job < jobs ? job / units * N : p.rows;
+        const int unit1 = job < jobs ? (int)(job % units) : 0;
+        fetch(next, row1, unit1);
+        float mine = 0.f;  // lane i of a block keeps row i's scale
 #pragma unroll
-            for (int a = 0; a < ACC; ++a) {
-                const int col = (u0 + u) * COLS + a * 32 * V + lane * V;
-                float t[V];
-                if (col < p.K) load_elems<T, V>(xr + col, t);
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[u][a * V + i] = col < p.K ? t[i] : 0.f;
-            }
-#pragma unroll
-        for (int u = 0; u < QUANT_UNITS; ++u) {
-            if (u0 + u >= units) break;
-            float amax = 0.f;
-#pragma unroll
-            for (int i = 0; i < EPT; ++i) amax = max_nan(amax, fabsf(v[u][i]));
-            amax = max_lanes<V == 8 ? 16 : 32>(amax);
-            const float scale = fp8_scale(amax);
-#pragma unroll
-            for (int a = 0; a < ACC; ++a) {
-                const int col = (u0 + u) * COLS + a * 32 * V + lane * V;
-                float t[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) t[i] = v[u][a * V + i];
-                if (col < p.K) store_fp8<V>(qr + col, t, scale);
-            }
-            const int first = (u0 + u) * COLS + lane * V;
-            if ((lane & (V == 8 ? 15 : 31)) == 0 && first < p.K)
-                p.scales[row * p.scale_row + (long long)(first / FP8_BLOCK) * p.scale_blk] = scale;
+        for (int i = 0; i < N; ++i) {
+            const float scale = fp8_scale(max_lanes<HALF>(now[i].amax()));
+            now[i].store(p.q + (row + i) * p.q_stride, unit, lane, row + i < p.rows ? p.K : 0, Fp8Scale(scale));
+            if ((lane & (HALF - 1)) == i) mine = scale;
         }
+        const int i = lane & (HALF - 1), block = unit * (U::COLS / FP8_BLOCK) + lane / HALF;
+        if (i < N && row + i < p.rows && block * FP8_BLOCK < p.K)
+            p.scales[(row + i) * p.scale_row + (long long)block * p.scale_blk] = mine;
+        if (job >= jobs) return;
+        row = row1;
+        unit = unit1;
+#pragma unroll
+        for (int k = 0; k < N; ++k) now[k] = next[k];
     }
 }
 
@@ -95,6 +142,7 @@ template <typename T, int V> __global__ void __launch_bounds__(256) quant_blocks
 #pragma unroll
     for (int k = 0; k < 8; ++k) amax = max_nan(amax, red[k]);
     const float scale = fp8_scale(amax);
+    const Fp8Scale by(scale);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
         const long long row = row0 + warp + 8 * r;
@@ -103,8 +151,8 @@ template <typename T, int V> __global__ void __launch_bounds__(256) quant_blocks
             const int col = col0 + a * 32 * V + lane * V;
             float t[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) t[i] = v[r][a * V + i];
-            if (row < p.rows && col < p.K) store_fp8<V>(p.q + row * p.q_stride + col, t, scale);
+            for (int i = 0; i < V; ++i) t[i] = -v[r][a * V + i];
+            if (row < p.rows && col < p.K) store_fp8<V>(p.q + row * p.q_stride + col, t, by);
         }
     }
     if (threadIdx.x == 0) p.scales[(long long)blockIdx.y * p.scale_row + (long long)blockIdx.x * p.scale_blk] = scale;
