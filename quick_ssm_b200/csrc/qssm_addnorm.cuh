@@ -27,10 +27,7 @@
 namespace qssm {
 
 constexpr int ADDNORM_WARPS = 8;      // warps per CTA
-
-
-
-constexpr int ADDNORM_HELD = 16;       // elements of a row that a lane holds in registers
+constexpr int ADDNORM_HELD = 16;      // elements of a row that a lane holds in registers
 constexpr int ADDNORM_CTAS = 4;       // upper bound of CTAs per SM in the backward (sizes its scratch)
 
 struct AddNormParams {

@@ -23,11 +23,16 @@ from . import _lib
 from .scan_interface import _addressable, _n_tiles, scan
 
 
-def _composed(pa, px, pc1, pc2, pd, gate_dtype, out_dtype):
+def _gates(pa, px, pc1, pc2, pd, gate_dtype):
     a = torch.sigmoid(pa).to(gate_dtype)
     x = px.to(gate_dtype)
     c = (F.silu(pc1) * pc2).to(gate_dtype)
     b = torch.sigmoid(pd).to(gate_dtype)
+    return a, x, c, b
+
+
+def _composed(pa, px, pc1, pc2, pd, gate_dtype, out_dtype):
+    a, x, c, b = _gates(pa, px, pc1, pc2, pd, gate_dtype)
     return scan(x=x, a=a, b=b, c=c, out_dtype=out_dtype)
 
 

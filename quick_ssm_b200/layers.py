@@ -87,18 +87,135 @@ class SSMFused(SSM):
         if backend == "torch" or x.device.type != "cuda" or not checkpoint:
             return super().forward(x, block_l=block_l, checkpoint=checkpoint, tile_b=tile_b, tile_d=tile_d,
                                    backend=backend, scan_out_dtype=scan_out_dtype)
-        from .gated import gated_scan
         skip = x if self.use_residual else 0
         if self.use_norm:  # the normalisation kernels on the layer's own weight
             from .norm import rms_norm
             u = rms_norm(x, self.pre_norm.weight, self.pre_norm.eps)
         else:
             u = x
+        return self._branch(u, scan_out_dtype) + skip
+
+    def _branch(self, u: torch.Tensor, scan_out_dtype: Optional[torch.dtype]) -> torch.Tensor:
+        """The block behind its pre-norm and in front of its residual."""
+        from .gated import gated_scan
         if scan_out_dtype is None:
             scan_out_dtype = self.out_proj.weight.dtype
         h = gated_scan(self.A_proj(u), self.B_proj(u), self.C_proj_a(u), self.C_proj_b(u), self.D_proj(u),
                        gate_dtype=self.compute_dtype, out_dtype=scan_out_dtype)
-        return self.out_proj(h.to(self.out_proj.weight.dtype)) + skip
+        return self.out_proj(h.to(self.out_proj.weight.dtype))
 
 
-__all__ = ["SSM", "SSMFused", "RMSNorm", "RMSNormFused"]
+class SSMStack(nn.Module):
+    """``n_layers`` residual SSM blocks, the same function as ``nn.Sequential`` of ``SSM`` with the same weights.
+    The residual stream and the blocks' outputs are kept apart between two blocks, so that the residual's addition and
+    the next block's norm are one kernel per direction (``norm.add_rms_norm``).  ``layers`` holds the blocks; a state
+    dict of such a ``Sequential`` loads with its keys prefixed by ``layers.``."""
+
+    def __init__(self, n_layers: int, hidden_size: int, state_size_mult: float = 1.0, eps: float = 1e-5,
+                 dtype: torch.dtype = torch.float32, device: Optional[torch.device] = None,
+                 compute_dtype: torch.dtype = torch.float16):
+        super().__init__()
+        self.layers = nn.ModuleList(SSMFused(hidden_size, state_size_mult, eps, dtype, device, compute_dtype)
+                                    for _ in range(n_layers))
+
+    def forward(self, x: torch.Tensor, *, backend: str = "auto",
+                scan_out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        if backend == "torch" or x.device.type != "cuda" or not self.layers:
+            for layer in self.layers:
+                x = layer(x, backend=backend, scan_out_dtype=scan_out_dtype)
+            return x
+        from .norm import add_rms_norm, rms_norm
+        first = self.layers[0]
+        h, y = x, first._branch(rms_norm(x, first.pre_norm.weight, first.pre_norm.eps), scan_out_dtype)
+        for layer in self.layers[1:]:
+            u, h = add_rms_norm(y, h, layer.pre_norm.weight, layer.pre_norm.eps)
+            y = layer._branch(u, scan_out_dtype)
+        return y + h
+
+
+class SSMFp8(nn.Module):
+    """An ``SSM`` block for serving, its projections in 8 bits (``fp8.matmul_fp8``): made from a trained block with
+    ``SSMFp8(block)``.  One pass is five kernels for a prompt and for a single token alike: residual sum, norm and
+    quantisation; the five input projections as one product; the scan with its gates and a carried state; quantisation;
+    the output projection.  No gradient.
+
+    ``forward(x, residual, state)`` takes the previous block's output and the residual stream apart (``residual=None``:
+    x is the stream itself) and returns ``(out, residual, state)``; the stream behind this block is ``out + residual``.
+    ``state`` is a ``streaming.ScanState`` or None at the start of a sequence."""
+
+    def __init__(self, block: SSM, gate_dtype: Optional[torch.dtype] = None):
+        super().__init__()
+        if not (block.use_norm and block.use_residual):
+            raise ValueError("SSMFp8 serves blocks with a pre-norm and a residual")
+        if block.A_proj.weight.device.type != "cuda":
+            raise RuntimeError("SSMFp8 needs a block on a CUDA device; there is no CPU path")
+        from .fp8 import quantize_weight
+        n = block.state_size_dim
+        self.state_size_dim, self.hidden_size, self.eps = n, block.hidden_size, block.pre_norm.eps
+        if gate_dtype is None:
+            gate_dtype = block.compute_dtype if block.compute_dtype != torch.float32 else torch.bfloat16
+        if gate_dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"gates are bfloat16 or float16; got {gate_dtype}")
+        self.gate_dtype = gate_dtype
+        with torch.no_grad():
+            w_in = quantize_weight(torch.cat([m.weight for m in (block.A_proj, block.B_proj, block.C_proj_a,
+                                                                 block.C_proj_b, block.D_proj)]))
+            w_out = quantize_weight(block.out_proj.weight)
+            bias = torch.zeros(5 * n, dtype=torch.float32, device=block.A_proj.weight.device)
+            bias[:n] = block.A_proj.bias
+            self._keep("in", w_in, bias)
+            self._keep("out", w_out, block.out_proj.bias.detach().float().clone())
+            self.register_buffer("norm_weight", block.pre_norm.weight.detach().clone())
+
+    def _keep(self, name: str, w, bias: torch.Tensor) -> None:
+        # bytes: the values' rows are spaced for the copy engine, and a state dict keeps them as they are
+        self.register_buffer(f"{name}_values", w.values.view(torch.uint8))
+        self.register_buffer(f"{name}_scales", w.scales)
+        self.register_buffer(f"{name}_bias", bias)
+
+    def _weight(self, name: str):
+        from .fp8 import Fp8Weight
+        return Fp8Weight(getattr(self, f"{name}_values").view(torch.float8_e4m3fn), getattr(self, f"{name}_scales"))
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, state=None):
+        from .fp8 import matmul_fp8, quantize_rows
+        from .norm import add_rms_norm_fp8
+        from .streaming import gated_scan_chunk
+        u, h = add_rms_norm_fp8(x, residual, self.norm_weight, self.eps)
+        p = matmul_fp8(u, self._weight("in"), self.in_bias, out_dtype=self.gate_dtype)
+        y, state = gated_scan_chunk(*p.split(self.state_size_dim, dim=-1), state)
+        out = matmul_fp8(quantize_rows(y), self._weight("out"), self.out_bias, out_dtype=self.gate_dtype)
+        return out, h, state
+
+
+class SSMStackFp8(nn.Module):
+    """A stack of ``SSM`` blocks (an ``SSMStack``, or any iterable of blocks) for serving in 8 bits.
+    ``forward(x, states)`` feeds ``[B, L, hidden]`` (a prompt, or the next token with ``L = 1``) and returns
+    ``(y, states)``: y in x's type, the states to pass with the next piece."""
+
+    def __init__(self, blocks, gate_dtype: Optional[torch.dtype] = None):
+        super().__init__()
+        self.layers = nn.ModuleList(SSMFp8(b, gate_dtype) for b in getattr(blocks, "layers", blocks))
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, states=None):
+        if states is None:
+            states = [None] * len(self.layers)
+        if len(states) != len(self.layers):
+            raise ValueError(f"{len(states)} states for {len(self.layers)} blocks")
+        if not self.layers:
+            return x, []
+        if x.dim() != 3:
+            raise ValueError("x must be [B, L, hidden]")
+        y, h, after = x, None, []
+        for layer, state in zip(self.layers, states):
+            # a residual stream in the branch's own type, or in fp32 under 16-bit branches
+            y, h, state = layer(y, h, state)
+            if h.dtype not in (y.dtype, torch.float32):
+                h = h.float()
+            after.append(state)
+        return (h + y).to(x.dtype), after
+
+
+__all__ = ["SSM", "SSMFused", "SSMStack", "SSMFp8", "SSMStackFp8", "RMSNorm", "RMSNormFused"]
