@@ -57,11 +57,11 @@ __device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) { return make_
 constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;        // a pair's tile
 constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
 constexpr int MMR_WARPS = 8, MMR_COLS = 128;                   // warps that hold sums, columns of each
-constexpr int MMR_THREADS = 32 * MMR_WARPS + 256;              // warp 8 copies, 9 to 12 products, 13 scales
+constexpr int MMR_THREADS = 32 * MMR_WARPS + 256;              // warp 8 copies, 9 to 12 products, 13 scales, 14 bias
 // Scales in flight: slots of four blocks, a block being 128 of x and two of w.
 constexpr int MMR_SLOTS = 4, MMR_GROUP = 4, MMR_BLOCK = 576, MMR_SLOT = MMR_GROUP * MMR_BLOCK;
 constexpr int MMR_OUT = MMR_STAGES * MMR_STAGE, MMR_BIAS = MMR_OUT + MMR_WARPS * 8192,
-              MMR_SCALES = MMR_BIAS + MMR_WARPS * MMR_COLS * 4, MMR_BARS = MMR_SCALES + MMR_SLOTS * MMR_SLOT,
+              MMR_SCALES = MMR_BIAS + 2 * MMR_N * 4, MMR_BARS = MMR_SCALES + MMR_SLOTS * MMR_SLOT,
               MMR_SMEM = MMR_BARS + 512 + 1024;
 // Registers: 128 a thread at launch (512 threads); the eight helper warps give 88 of theirs to the eight others.
 constexpr int MMR_REGS_SUMS = 216, MMR_REGS_HELP = 40;
@@ -88,8 +88,9 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     const uint32_t base = smem_u32(smem), bars = base + MMR_BARS;
     // full, taken: the even CTA's count for both; the others are each CTA's own.  Buffer b = 2 * (block & 1) + half.
     const uint32_t full = bars, empty = full + 8 * MMR_STAGES, done = empty + 8 * MMR_STAGES, taken = done + 32,
-                   scaled = taken + 32, used = scaled + 8 * MMR_SLOTS, last = used + 8 * MMR_SLOTS;
-    static_assert(8 * (2 * MMR_STAGES + 8 + 2 * MMR_SLOTS + 1) + 4 <= 512, "room for the barriers");
+                   scaled = taken + 32, used = scaled + 8 * MMR_SLOTS, biased = used + 8 * MMR_SLOTS,
+                   unbiased = biased + 16, last = unbiased + 16;
+    static_assert(8 * (2 * MMR_STAGES + 8 + 2 * MMR_SLOTS + 5) + 4 <= 512, "room for the barriers");
     volatile uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + (last + 8 - base));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -97,6 +98,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
         for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 2); }  // empty: both halves
         for (int b = 0; b < 4; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, MMR_WARPS); }
         for (int f = 0; f < MMR_SLOTS; ++f) { mbar_init(scaled + 8 * f, 32); mbar_init(used + 8 * f, MMR_WARPS); }
+        for (int i = 0; i < 2; ++i) { mbar_init(biased + 8 * i, 1); mbar_init(unbiased + 8 * i, MMR_WARPS); }
         mbar_init(last, 4);
         fence_barrier_init();
     }
@@ -185,30 +187,44 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                 }
             }
             copies_wait();
+        } else if (warp == MMR_WARPS + 6 && p.bias != nullptr) {  // the next tile's bias while this one is worked on
+            uint32_t turn = 0;
+            for (int t = pair; ok && t < tiles; t += pairs, ++turn) {
+                const int n0 = (t / p.m_tiles) * MMR_N;
+                float v[MMR_N / 32];
+#pragma unroll
+                for (int i = 0; i < MMR_N / 32; ++i) v[i] = load_bias(p, n0 + 32 * i + lane);
+                if (turn >= 2) ok = mbar_wait_limit(unbiased + 8 * (turn & 1), ((turn >> 1) - 1) & 1);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                float* to = reinterpret_cast<float*>(smem + MMR_BIAS) + (turn & 1) * MMR_N;
+#pragma unroll
+                for (int i = 0; i < MMR_N / 32; ++i) to[32 * i + lane] = v[i];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(biased + 8 * (turn & 1));
+            }
         }
     } else {
         regs_up<MMR_REGS_SUMS>();
         const int quarter = warp & 3, half = warp >> 2, col0 = half * MMR_COLS;
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
         const uint32_t taken0 = cluster_addr(taken, 0) + 8 * half, my_done = done + 8 * half;
-        float* my_bias = reinterpret_cast<float*>(smem + MMR_BIAS) + warp * MMR_COLS;
         const float* my_x = reinterpret_cast<const float*>(smem + MMR_SCALES) + quarter * 32 + lane;
         const float* my_w = reinterpret_cast<const float*>(smem + MMR_SCALES) + 128 + half;
-        uint32_t it = 0;
-        for (int t = pair; ok && t < tiles; t += pairs) {
+        uint32_t it = 0, turn = 0;
+        for (int t = pair; ok && t < tiles; t += pairs, ++turn) {
             const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + quarter * 32, n0 = (t / p.m_tiles) * MMR_N + col0;
             float2 acc[MMR_COLS / 2];
             if (p.bias != nullptr) {  // the sums start from the bias
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < MMR_COLS; i += 32) my_bias[i + lane] = load_bias(p, n0 + i + lane);
-                __syncwarp();
+                ok = mbar_wait_limit(biased + 8 * (turn & 1), (turn >> 1) & 1);
+                const float* bias = reinterpret_cast<const float*>(smem + MMR_BIAS) + (turn & 1) * MMR_N + col0;
 #pragma unroll
                 for (int j = 0; j < MMR_COLS / 4; ++j) {
-                    const float4 v = *reinterpret_cast<const float4*>(my_bias + 4 * j);
+                    const float4 v = *reinterpret_cast<const float4*>(bias + 4 * j);
                     acc[2 * j] = make_float2(v.x, v.y);
                     acc[2 * j + 1] = make_float2(v.z, v.w);
                 }
+                __syncwarp();
+                if (lane == 0 && ok) mbar_arrive(unbiased + 8 * (turn & 1));
             } else {
 #pragma unroll
                 for (int j = 0; j < MMR_COLS / 2; ++j) acc[j] = make_float2(0.f, 0.f);
