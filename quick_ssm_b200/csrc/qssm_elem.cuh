@@ -18,6 +18,17 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two values rounded and packed in one conversion.
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
 template <int BYTES> struct Word;
 template <> struct Word<2> { using type = uint16_t; };
 template <> struct Word<4> { using type = uint32_t; };
@@ -51,9 +62,14 @@ template <typename T, int V> __device__ __forceinline__ void store_elems(T* p, c
         store_elems<T, V / 2>(p, lo);
         store_elems<T, V / 2>(p + V / 2, hi);
     } else {
-        union U { typename Word<BYTES>::type w; T e[V]; __device__ U() {} } u;
+        union U { typename Word<BYTES>::type w; T e[V]; uint32_t p[V > 1 ? V / 2 : 1]; __device__ U() {} } u;
+        if constexpr (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
+            for (int i = 0; i < V / 2; ++i) u.p[i] = pack_pair<T>(v[2 * i], v[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
+        }
         *reinterpret_cast<typename Word<BYTES>::type*>(p) = u.w;
     }
 }

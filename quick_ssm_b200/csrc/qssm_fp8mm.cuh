@@ -265,36 +265,44 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
             // 128 bytes of each row at a time; 16-byte piece c of row r lies at c ^ (r & 7), where a bulk store in the
             // 128-byte swizzle looks for it, and eight lanes' pieces in eight different banks
             constexpr int V = 16 / sizeof(T), COLS = 8 * V, CHUNKS = MMR_COLS / COLS;
+            uint8_t* const bufs = smem + MMR_OUT + warp * 8192;
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) {
-                uint8_t* const buf = smem + MMR_OUT + warp * 8192 + (c & 1) * 4096;
-                if (lane == 0) tma_wait_read<1>();  // the store that read this buffer before
+            for (int c0 = 0; c0 < CHUNKS; c0 += 2) {  // two pieces behind one fence
+                if (lane == 0) tma_wait_read<0>();  // the stores that read these buffers before
                 __syncwarp();
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    float v[V];
+                for (int c = c0; c < c0 + 2; ++c)
 #pragma unroll
-                    for (int i = 0; i < V; i += 2) {
-                        v[i] = acc[(c * COLS + q * V + i) / 2].x;
-                        v[i + 1] = acc[(c * COLS + q * V + i) / 2].y;
+                    for (int q = 0; q < 8; ++q) {
+                        float v[V];
+#pragma unroll
+                        for (int i = 0; i < V; i += 2) {
+                            v[i] = acc[(c * COLS + q * V + i) / 2].x;
+                            v[i + 1] = acc[(c * COLS + q * V + i) / 2].y;
+                        }
+                        store_elems<T, V>(reinterpret_cast<T*>(bufs + (c - c0) * 4096 + lane * 128 + ((q ^ (lane & 7)) << 4)), v);
                     }
-                    store_elems<T, V>(reinterpret_cast<T*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)), v);
-                }
                 if (p.y_vec) {
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        if (n0 + c * COLS < p.N) tma_store_2d(&p.y_map, smem_u32(buf), n0 + c * COLS, m0);
+                        if (n0 + c0 * COLS < p.N) tma_store_2d(&p.y_map, smem_u32(bufs), n0 + c0 * COLS, m0);
+                        if (n0 + (c0 + 1) * COLS < p.N) tma_store_2d(&p.y_map, smem_u32(bufs) + 4096, n0 + (c0 + 1) * COLS, m0);
                         tma_commit();
                     }
                 } else {  // rows of y on any boundary: each row's 128 bytes by consecutive lanes, in the words that fit
                     __syncwarp();
-                    const int rows = p.M - m0 < 32 ? p.M - m0 : 32, bytes = (p.N - n0 - c * COLS) * (int)sizeof(T);
-                    uint8_t* dst = static_cast<uint8_t*>(p.y) + ((long long)m0 * p.y_stride + n0 + c * COLS) * sizeof(T);
+                    const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
                     const long long pitch = p.y_stride * sizeof(T);
-                    if (p.y_word == 8) put_rows<8>(buf, dst, pitch, rows, bytes, lane);
-                    else if (p.y_word == 4) put_rows<4>(buf, dst, pitch, rows, bytes, lane);
-                    else put_rows<2>(buf, dst, pitch, rows, bytes, lane);
+#pragma unroll
+                    for (int c = c0; c < c0 + 2; ++c) {
+                        const int bytes = (p.N - n0 - c * COLS) * (int)sizeof(T);
+                        const uint8_t* buf = bufs + (c - c0) * 4096;
+                        uint8_t* dst = static_cast<uint8_t*>(p.y) + ((long long)m0 * p.y_stride + n0 + c * COLS) * sizeof(T);
+                        if (p.y_word == 8) put_rows<8>(buf, dst, pitch, rows, bytes, lane);
+                        else if (p.y_word == 4) put_rows<4>(buf, dst, pitch, rows, bytes, lane);
+                        else put_rows<2>(buf, dst, pitch, rows, bytes, lane);
+                    }
                 }
             }
         }
