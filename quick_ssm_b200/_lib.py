@@ -450,18 +450,21 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 def _ordinal(first: torch.Tensor, *others) -> int:
     """Device ordinal that all tensors (None is skipped) share."""
-    index = first.get_device() if first.is_cuda else -1
-    if index < 0:
-        raise RuntimeError("the qssm kernels need CUDA tensors; there is no CPU path")
+    index = first.get_device()
     for t in others:
-        if t is not None and (not t.is_cuda or t.get_device() != index):
-            _require_cuda(first, *others)
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        _require_cuda(first, *others)  # says which of the two it is
     return index
+
+
+_current_device = torch.cuda.current_device
 
 
 def _call(fn, name: str, index: int, args) -> None:
     """``fn(*args, stream)`` with device ``index`` current."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -497,14 +500,20 @@ def add_rmsnorm_fp8(x, res, w, q, scales, h, eps: float) -> None:
            srow, sblk, eps, code, rcode, _DTYPE_CODE[w.dtype]))
 
 
+_norm_parts = {}   # device ordinal -> partial sums of dw
+
+
 def add_rmsnorm_bwd(h, w, dy, dh, rstd, dx, dres, dw) -> None:
     """Gradients of ``add_rmsnorm_fwd``; dh, dx, dres may be None (not both of the last two)."""
     index = _ordinal(h, dy, dh)
     lib = _lib or load()
     rows, H = h.shape
-    with _on_device(h.device):
-        nbytes = int(lib.qssm_add_rmsnorm_workspace_bytes(rows, H))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
+    most = _norm_parts.get(index)
+    if most is None:
+        with _on_device(h.device):  # rows of scratch that a call on this device takes at most
+            most = _norm_parts[index] = int(lib.qssm_add_rmsnorm_workspace_bytes(1 << 40, 1)) // 4
+    nbytes = 4 * min(rows, most) * H
+    ws = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=h.device)
 
     def at(t):
         return (None, 0) if t is None else (t.data_ptr(), t.stride(0))

@@ -96,6 +96,7 @@ MatmulPlan plan_matmul(long long M, long long N, int n_kb, double ragged_us) {
     const int T = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const double per_block = T == 16 ? 0.35 : T == 32 ? 0.4 : T == 64 ? 0.5 : 0.65;
     const long long tiles = ((N + 127) / 128) * ((M + T - 1) / T);
+    if ((M + T - 1) / T > 65535) return plan;  // more tiles of rows than a grid has in its second direction
     for (int S = 1; S <= 8 && S <= n_kb; S *= 2) {
         const long long seats = (T <= 64 ? 2 : 1) * (S == 8 ? sms * 3 / 4 : S == 4 ? sms * 11 / 12 : sms);
         const double cost = 4.0 + (double)((tiles * S + seats - 1) / seats) * (per_block * ((n_kb + S - 1) / S) + 1.0) +
@@ -113,7 +114,7 @@ template <typename OUT, int T> int launch_few(const MatmulParams& p, int S, cuda
     const int rc = ensure_smem(kernel, Few<T>::SMEM);
     if (rc) return rc;
     const long long gx = (long long)((p.N + 127) / 128) * S, gy = (p.M + T - 1) / T;
-    if (gx >= (1ll << 31) || gy > 65535) return QSSM_E_SHAPE;
+    if (gx >= (1ll << 31)) return QSSM_E_SHAPE;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)gx, (unsigned)gy);

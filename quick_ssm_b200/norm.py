@@ -81,23 +81,21 @@ def _check_add(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.
             raise TypeError(f"residual must be in x's type or in float32; got {residual.dtype} with x in {dt}")
 
 
-def _dense(shape, dtype, device) -> torch.Tensor:
-    """An uninitialised contiguous tensor (``empty_strided`` takes two thirds of ``empty``'s time on the host)."""
-    strides, step = [], 1
-    for n in reversed(shape):
-        strides.append(step)
-        step *= max(n, 1)
-    return torch.empty_strided(tuple(shape), strides[::-1], dtype=dtype, device=device)
+def _room_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape (``empty_like`` takes half of ``empty``'s time on the host)."""
+    if t.dtype is dtype and t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
 class _AddRMSNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
         x2, r2, w = rows_2d(x), rows_2d(residual), weight.contiguous()
-        dev = x.device
-        y = _dense(x.shape, x.dtype, dev)
-        h = _dense(x.shape, residual.dtype, dev)
-        rstd = torch.empty(x2.shape[0], dtype=torch.float32, device=dev) if any(ctx.needs_input_grad) else None
+        y = _room_like(x, x.dtype)
+        h = _room_like(residual, residual.dtype)
+        rstd = torch.empty_strided((x2.shape[0],), (1,), dtype=torch.float32, device=x.device) \
+            if any(ctx.needs_input_grad) else None
         _lib.add_rmsnorm_fwd(x2, r2, w, rows_2d(y), rows_2d(h), rstd, eps)
         if rstd is not None:
             ctx.save_for_backward(h, w, rstd)
@@ -113,10 +111,10 @@ class _AddRMSNormFunction(torch.autograd.Function):
         if dy is None:  # only h was used: its gradient passes through
             return (dh if need_x else None), (dh if need_r else None), None, None
         # autograd hands over gradients in the outputs' types and takes the inputs' own back
-        xd, rd, dev, shape = dy.dtype, h.dtype, h.device, h.shape
-        dx = _dense(shape, xd, dev) if need_x or rd is xd else None
-        dres = _dense(shape, rd, dev) if rd is not xd and (need_r or dx is None) else None
-        dw = _dense(w.shape, w.dtype, dev)
+        xd, rd = dy.dtype, h.dtype
+        dx = _room_like(h, xd) if need_x or rd is xd else None
+        dres = torch.empty_like(h) if rd is not xd and (need_r or dx is None) else None
+        dw = torch.empty_like(w)
         _lib.add_rmsnorm_bwd(rows_2d(h), w, rows_2d(dy), None if dh is None else rows_2d(dh), rstd,
                              None if dx is None else rows_2d(dx), None if dres is None else rows_2d(dres), dw)
         return (dx if need_x else None), ((dx if rd is xd else dres) if need_r else None), (dw if need_w else None), None
@@ -149,6 +147,6 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
         h = x
         _lib.add_rmsnorm_fp8(x2, None, w, q.values, q.scales, None, float(eps))
     else:
-        h = _dense(x.shape, residual.dtype, x.device)
+        h = _room_like(residual, residual.dtype)
         _lib.add_rmsnorm_fp8(x2, rows_2d(residual), w, q.values, q.scales, rows_2d(h), float(eps))
     return q._under(x.shape), h

@@ -278,6 +278,28 @@ def test_product_is_deterministic_and_leaves_its_neighbours_alone():
         assert torch.isnan(y[0]).all() and torch.equal(y[1:], a[1:])
 
 
+@gpu
+def test_product_of_more_rows_than_a_grid_has_in_one_direction():
+    M, N, K = 8_400_000, 1, 16
+    x = fp8.quantize_rows(torch.randn(M, K, device="cuda"))
+    w = fp8.quantize_weight(torch.randn(N, K, device="cuda"))
+    y = fp8.matmul_fp8(x, w, out_dtype=F32)
+    at = torch.cat([torch.arange(0, M, 4099), torch.arange(M - 300, M)])
+    part = fp8.Fp8Rows(x.values[at.cuda()], x.scales[at.cuda()])
+    check_product(y[at.cuda()], part, w, None)
+    assert torch.isfinite(y).all()
+
+
+@gpu
+def test_scales_shared_by_broadcasting():
+    """One scale for a whole operand, expanded: strides of zero."""
+    x, w, _ = operands(300, 520, 700)
+    xs, ws = torch.full((1, 1), 0.25, device="cuda").expand(300, 6), torch.full((1, 1), 0.5, device="cuda").expand(5, 6)
+    for rows in (3, 300):
+        part = fp8.Fp8Rows(x.values[:rows], xs[:rows])
+        check_product(fp8.matmul_fp8(part, fp8.Fp8Weight(w.values, ws), out_dtype=F32), part, fp8.Fp8Weight(w.values, ws), None)
+
+
 # ------------------------------------------------------------------------------------------------
 # residual norm
 # ------------------------------------------------------------------------------------------------
