@@ -132,6 +132,10 @@ struct Fp8Scale {
         r = fmaf(fmaf(-s, e, 1.f), e, e);
         if (!(scale < 3.402823466e38f)) r = scale == scale ? 0.f : scale;
     }
+    __device__ __forceinline__ Fp8Scale(float s_, float r_) : s(s_), r(r_) {}
+    __device__ __forceinline__ Fp8Scale from_lane(int lane) const {
+        return Fp8Scale(__shfl_sync(0xffffffffu, s, lane), __shfl_sync(0xffffffffu, r, lane));
+    }
     // v / scale from -v (so that a zero keeps its sign and two values go through one instruction)
     __device__ __forceinline__ float of_negated(float nv) const {
         const float q = nv * -r;
