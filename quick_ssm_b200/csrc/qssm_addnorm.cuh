@@ -190,6 +190,25 @@ __device__ __forceinline__ void put_units_fp8(const AddNormParams& p, long long 
     if (lane < NB && block * FP8_BLOCK < p.H) p.scales[row * p.scale_row + (long long)block * p.scale_blk] = scale;
 }
 
+// A unit of a row as it lies in memory (16-bit elements two to a register).
+template <typename T, int V> struct Packed {
+    static constexpr int EPT = Unit<V>::EPT;
+    alignas(16) T e[EPT];
+    __device__ __forceinline__ void load(const T* row, int unit, int lane, int cols) {
+        constexpr int BYTES = V * (int)sizeof(T) > 16 ? 16 : V * (int)sizeof(T), WORDS = EPT * (int)sizeof(T) / BYTES,
+                      PER_ACC = WORDS / Unit<V>::ACC;
+        using W = typename Word<BYTES>::type;
+        W* w = reinterpret_cast<W*>(e);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            const int col = Unit<V>::col(unit, i / PER_ACC, lane) + (i % PER_ACC) * (BYTES / (int)sizeof(T));
+            w[i] = W{};
+            if (col < cols) w[i] = *reinterpret_cast<const W*>(row + col);
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return to_f32(e[i]); }
+};
+
 // WPR: warps per row.  NU: units of a row held in registers by each of its warps, 0 for rows that are longer.  R: rows at
 // a time.
 template <typename TX, typename TR, int V, int WPR, int NU, int R, bool FP8>
@@ -208,33 +227,39 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
 #pragma unroll
         for (int u = 0; u < N; ++u) load_weight<V>(p, u * WPR + wid, lane, w[u]);
     }
-    for (long long row0 = ((long long)blockIdx.x * ROWS + warp / WPR) * R; row0 < p.rows; row0 += step) {
+    // rows held in registers: the next ones are on their way while these are worked on
+    Packed<TX, V> x[R][N], x_next[R][N];
+    Packed<TR, V> res[R][N], res_next[R][N];
+    auto fetch = [&](Packed<TX, V> (&xi)[R][N], Packed<TR, V> (&ri)[R][N], long long row0) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const long long row = row0 + k;
+            const int cols = row < p.rows ? H : 0;
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                xi[k][u].load(static_cast<const TX*>(p.x) + row * p.x_stride, u * WPR + wid, lane, cols);
+                if (p.res != nullptr)
+                    ri[k][u].load(static_cast<const TR*>(p.res) + row * p.res_stride, u * WPR + wid, lane, cols);
+            }
+        }
+    };
+    const long long begin = ((long long)blockIdx.x * ROWS + warp / WPR) * R;
+    if constexpr (NU > 0) fetch(x, res, begin);
+    for (long long row0 = begin; row0 < p.rows; row0 += step) {
         if constexpr (NU > 0) {
+            fetch(x_next, res_next, row0 + step);
             float h[R][N][EPT];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
-                const TX* xr = static_cast<const TX*>(p.x) + (row0 + k) * p.x_stride;
-                const int cols = R == 1 || row0 + k < p.rows ? H : 0;
+                TR* hr = static_cast<TR*>(p.h) + (row0 + k) * p.h_stride;
+                const int cols = row0 + k < p.rows ? H : 0;
 #pragma unroll
-                for (int u = 0; u < N; ++u) load_unit<TX, V>(xr, u * WPR + wid, lane, cols, h[k][u]);
-            }
-            if (p.res != nullptr) {
-                float t[R][N][EPT];
+                for (int u = 0; u < N; ++u) {
 #pragma unroll
-                for (int k = 0; k < R; ++k) {
-                    const TR* rr = static_cast<const TR*>(p.res) + (row0 + k) * p.res_stride;
-                    const int cols = R == 1 || row0 + k < p.rows ? H : 0;
+                    for (int i = 0; i < EPT; ++i) h[k][u][i] = x[k][u][i];
+                    if (p.res != nullptr) {
 #pragma unroll
-                    for (int u = 0; u < N; ++u) load_unit<TR, V>(rr, u * WPR + wid, lane, cols, t[k][u]);
-                }
-#pragma unroll
-                for (int k = 0; k < R; ++k) {
-                    TR* hr = static_cast<TR*>(p.h) + (row0 + k) * p.h_stride;
-                    const int cols = R == 1 || row0 + k < p.rows ? H : 0;
-#pragma unroll
-                    for (int u = 0; u < N; ++u) {
-#pragma unroll
-                        for (int i = 0; i < EPT; ++i) h[k][u][i] = to_f32(from_f32<TR>(h[k][u][i] + t[k][u][i]));
+                        for (int i = 0; i < EPT; ++i) h[k][u][i] = to_f32(from_f32<TR>(h[k][u][i] + res[k][u][i]));
                         store_unit<TR, V>(hr, u * WPR + wid, lane, cols, h[k][u]);
                     }
                 }
@@ -259,6 +284,13 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
                 }
                 if constexpr (FP8) put_units_fp8<V, WPR>(p, row0 + k, wid, lane, h[k]);
             }
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                    x[k][u] = x_next[k][u];
+                    res[k][u] = res_next[k][u];
+                }
         } else {
             const TX* xr = static_cast<const TX*>(p.x) + row0 * p.x_stride;
             const TR* rr = static_cast<const TR*>(p.res) + row0 * p.res_stride;
@@ -294,25 +326,6 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
         }
     }
 }
-
-// A unit of a row as it lies in memory (16-bit elements two to a register).
-template <typename T, int V> struct Packed {
-    static constexpr int EPT = Unit<V>::EPT;
-    alignas(16) T e[EPT];
-    __device__ __forceinline__ void load(const T* row, int unit, int lane, int cols) {
-        constexpr int BYTES = V * (int)sizeof(T) > 16 ? 16 : V * (int)sizeof(T), WORDS = EPT * (int)sizeof(T) / BYTES,
-                      PER_ACC = WORDS / Unit<V>::ACC;
-        using W = typename Word<BYTES>::type;
-        W* w = reinterpret_cast<W*>(e);
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            const int col = Unit<V>::col(unit, i / PER_ACC, lane) + (i % PER_ACC) * (BYTES / (int)sizeof(T));
-            w[i] = W{};
-            if (col < cols) w[i] = *reinterpret_cast<const W*>(row + col);
-        }
-    }
-    __device__ __forceinline__ float operator[](int i) const { return to_f32(e[i]); }
-};
 
 // Backward.  Each warp keeps the dw sums of its columns: in registers over all its rows (NU > 0), added up over the
 // CTA's row groups in order at the end; for longer rows (eight warps each) in the CTA's part of the scratch.  What a row
