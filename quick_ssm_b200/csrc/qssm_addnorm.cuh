@@ -19,8 +19,9 @@
 //
 // A row is held by 1, 2, 4 or 8 warps, 16 elements a lane (the backward keeps three values of each, packed as they came,
 // and the dw sums), which leaves room for 16 to 32 warps on an SM; a warp takes several rows of one unit at a time.
-// Measured on a B200 against the copy rate (6.54 TB/s), bf16 65536x1024: forward 88 us of 82, to e4m3 107 of 72,
-// backward 113 of 82 (32 elements a lane as floats, eight warps on an SM: 187); fp32 165 of 164, 140 of 133, 167 of 164.
+// Measured on a B200 against the copy rate (6.54 TB/s), bf16 65536x1024: forward 88 us of 82, to e4m3 82 of 72,
+// backward 105 of 82 (32 elements a lane as floats, eight warps on an SM: 187; the next row not fetched ahead: 113, and
+// to e4m3 104); fp32 166 of 164, 132 of 133, 167 of 164.
 #pragma once
 #include "qssm_elem.cuh"
 
@@ -351,26 +352,39 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
     if constexpr (NU == 0) {
         for (int u = wid; u < units; u += WPR) store_unit<float, V>(part, u, lane, H, dw[0]);
     }
-    for (long long row0 = ((long long)blockIdx.x * ROWS + warp / WPR) * R; row0 < p.rows; row0 += step) {
-        if constexpr (NU > 0) {
-            Packed<TR, V> h[R][N], e[R][N];
-            Packed<TX, V> g[R][N];
-            float r[R];
+    // 16-bit rows: the next ones are on their way while these are worked on (with fp32 three more rows of registers cost
+    // more warps than that brings)
+    constexpr bool AHEAD = sizeof(TR) == 2 && NU > 0;
+    struct Rows {
+        Packed<TR, V> h[R][N], e[R][N];
+        Packed<TX, V> g[R][N];
+        float r[R];
+    };
+    auto fetch = [&](Rows& to, long long row0) {
 #pragma unroll
-            for (int k = 0; k < R; ++k) {
-                const long long row = row0 + k;
-                const int cols = R == 1 || row < p.rows ? H : 0;
-                r[k] = cols > 0 ? p.rstd[row] : 0.f;
+        for (int k = 0; k < R; ++k) {
+            const long long row = row0 + k;
+            const int cols = row < p.rows ? H : 0, ecols = p.dh != nullptr ? cols : 0;
+            to.r[k] = cols > 0 ? p.rstd[row] : 0.f;
 #pragma unroll
-                for (int u = 0; u < N; ++u) {
-                    h[k][u].load(static_cast<const TR*>(p.h) + row * p.h_stride, u * WPR + wid, lane, cols);
-                    g[k][u].load(static_cast<const TX*>(p.dy) + row * p.dy_stride, u * WPR + wid, lane, cols);
-                }
-                const int ecols = p.dh != nullptr ? cols : 0;
-#pragma unroll
-                for (int u = 0; u < N; ++u)
-                    e[k][u].load(static_cast<const TR*>(p.dh) + row * p.dh_stride, u * WPR + wid, lane, ecols);
+            for (int u = 0; u < N; ++u) {
+                to.h[k][u].load(static_cast<const TR*>(p.h) + row * p.h_stride, u * WPR + wid, lane, cols);
+                to.g[k][u].load(static_cast<const TX*>(p.dy) + row * p.dy_stride, u * WPR + wid, lane, cols);
+                to.e[k][u].load(static_cast<const TR*>(p.dh) + row * p.dh_stride, u * WPR + wid, lane, ecols);
             }
+        }
+    };
+    const long long begin = ((long long)blockIdx.x * ROWS + warp / WPR) * R;
+    Rows now, next;
+    if constexpr (AHEAD) fetch(now, begin);
+    for (long long row0 = begin; row0 < p.rows; row0 += step) {
+        if constexpr (NU > 0) {
+            if constexpr (AHEAD) fetch(next, row0 + step);
+            else fetch(now, row0);
+            auto& h = now.h;
+            auto& e = now.e;
+            auto& g = now.g;
+            auto& r = now.r;
             float dot[R];
 #pragma unroll
             for (int k = 0; k < R; ++k) dot[k] = 0.f;
@@ -395,7 +409,7 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
 #pragma unroll
                 for (int k = 0; k < R; ++k) {
                     const long long row = row0 + k;
-                    const int cols = R == 1 || row < p.rows ? H : 0;
+                    const int cols = row < p.rows ? H : 0;
                     float d[EPT];
 #pragma unroll
                     for (int i = 0; i < EPT; ++i)
@@ -406,6 +420,7 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
                         store_unit<TR, V>(static_cast<TR*>(p.dres) + row * p.dres_stride, u * WPR + wid, lane, cols, d);
                 }
             }
+            if constexpr (AHEAD) now = next;
         } else {
             const TR* hr = static_cast<const TR*>(p.h) + row0 * p.h_stride;
             const TX* gr = static_cast<const TX*>(p.dy) + row0 * p.dy_stride;
