@@ -125,7 +125,7 @@ template <int WPR> __device__ __forceinline__ float sum_row(float v, float (*red
     return v;
 }
 
-// One unit of y, 16/32 bits, or quantised (then -y is given): the lanes of a block agree on its largest magnitude.
+// One unit of y, 16/32 bits, or quantised: the lanes of a block agree on its largest magnitude.
 template <typename TX, int V, bool FP8, int EPT>
 __device__ __forceinline__ void put_unit(const AddNormParams& p, long long row, int unit, int lane, const float (&y)[EPT]) {
     if constexpr (!FP8) {
@@ -152,7 +152,7 @@ __device__ __forceinline__ void put_unit(const AddNormParams& p, long long row, 
     }
 }
 
-// All units that a warp holds of a row, quantised (-y is given).  Every lane learns all blocks' largest magnitudes; one
+// All units that a warp holds of a row, quantised.  Every lane learns all blocks' largest magnitudes; one
 // lane for each block turns its own into the scale, which saves the others that arithmetic (60 instructions of 29 for
 // four units of 128 columns).
 template <int V, int WPR, int N, int EPT>
@@ -274,9 +274,8 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
                     for (int i = 0; i < EPT; ++i) ss = fmaf(h[k][u][i], h[k][u][i], ss);
                 ss = sum_row<WPR>(ss, red, turn);
                 if (R > 1 && row0 + k >= p.rows) break;
-                float r = 1.f / sqrtf(ss * inv_h + p.eps);
+                const float r = 1.f / sqrtf(ss * inv_h + p.eps);
                 if (p.rstd != nullptr && lane == 0 && wid == 0) p.rstd[row0 + k] = r;
-                if constexpr (FP8) r = -r;
 #pragma unroll
                 for (int u = 0; u < N; ++u) {
 #pragma unroll
@@ -312,9 +311,8 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
                 for (int i = 0; i < EPT; ++i) ss = fmaf(h[i], h[i], ss);
             }
             ss = sum_row<WPR>(ss, red, turn);
-            float r = 1.f / sqrtf(ss * inv_h + p.eps);
+            const float r = 1.f / sqrtf(ss * inv_h + p.eps);
             if (p.rstd != nullptr && lane == 0 && wid == 0) p.rstd[row0] = r;
-            if constexpr (FP8) r = -r;
             for (int u = wid; u < units; u += WPR) {  // a lane reads back what it wrote itself
                 float h[EPT], wu[EPT];
                 if (p.res != nullptr) load_unit<TR, V>(hr, u, lane, H, h);

@@ -136,30 +136,35 @@ struct Fp8Scale {
     __device__ __forceinline__ Fp8Scale from_lane(int lane) const {
         return Fp8Scale(__shfl_sync(0xffffffffu, s, lane), __shfl_sync(0xffffffffu, r, lane));
     }
-    // v / scale from -v (so that a zero keeps its sign and two values go through one instruction)
-    __device__ __forceinline__ float of_negated(float nv) const {
-        const float q = nv * -r;
-        return fmaf(fmaf(q, s, nv), -r, q);
+    // -v / scale: in these signs a zero keeps its own, and two values go through one instruction
+    __device__ __forceinline__ float minus_of(float v) const {
+        const float q = v * -r;
+        return fmaf(fmaf(q, s, v), -r, q);
     }
-    __device__ __forceinline__ float2 of_negated(float2 nv) const {
+    __device__ __forceinline__ float2 minus_of(float2 v) const {
         const float2 nr = make_float2(-r, -r), s2 = make_float2(s, s);
         float2 q, e;
-        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(as_u64(q)) : "l"(as_u64(nv)), "l"(as_u64(nr)));
-        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(as_u64(e)) : "l"(as_u64(q)), "l"(as_u64(s2)), "l"(as_u64(nv)));
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(as_u64(q)) : "l"(as_u64(v)), "l"(as_u64(nr)));
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(as_u64(e)) : "l"(as_u64(q)), "l"(as_u64(s2)), "l"(as_u64(v)));
         asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(as_u64(q)) : "l"(as_u64(e)), "l"(as_u64(nr)));
         return q;
     }
 };
 
-// The quantised values of -nv.
-template <int V> __device__ __forceinline__ void store_fp8(uint8_t* p, const float (&nv)[V], const Fp8Scale& scale) {
+// Quantised values; the sign that `minus_of` turns is turned back in the bytes.
+template <int V> __device__ __forceinline__ void store_fp8(uint8_t* p, const float (&v)[V], const Fp8Scale& scale) {
     if constexpr (V == 1) {
-        *p = __nv_cvt_float_to_fp8(scale.of_negated(nv[0]), __NV_SATFINITE, __NV_E4M3);
+        *p = __nv_cvt_float_to_fp8(scale.minus_of(v[0]), __NV_SATFINITE, __NV_E4M3) ^ 0x80;
     } else {
-        union { typename Word<V>::type w; uint16_t h[V / 2]; } u;
+        union { typename Word<V>::type w; uint16_t h[V / 2]; uint32_t u[V < 4 ? 1 : V / 4]; } u;
 #pragma unroll
         for (int i = 0; i < V / 2; ++i)
-            u.h[i] = __nv_cvt_float2_to_fp8x2(scale.of_negated(make_float2(nv[2 * i], nv[2 * i + 1])), __NV_SATFINITE, __NV_E4M3);
+            u.h[i] = __nv_cvt_float2_to_fp8x2(scale.minus_of(make_float2(v[2 * i], v[2 * i + 1])), __NV_SATFINITE, __NV_E4M3);
+        if constexpr (V == 2) u.h[0] ^= 0x8080u;
+        else {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) u.u[i] ^= 0x80808080u;
+        }
         *reinterpret_cast<typename Word<V>::type*>(p) = u.w;
     }
 }

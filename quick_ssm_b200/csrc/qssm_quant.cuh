@@ -53,18 +53,9 @@ template <typename T, int V> struct QuantUnit {
 #pragma unroll
         for (int a = 0; a < ACC; ++a) {
             const int col = unit * COLS + a * 32 * V + lane * V;
-            alignas(16) T ne[V];  // negated, 16-bit types two at a time
-            if constexpr (sizeof(T) == 2 && V >= 2) {
-#pragma unroll
-                for (int i = 0; i < V / 2; ++i)
-                    reinterpret_cast<uint32_t*>(ne)[i] = reinterpret_cast<const uint32_t*>(e + a * V)[i] ^ 0x80008000u;
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) ne[i] = -e[a * V + i];
-            }
             float t[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) t[i] = to_f32(ne[i]);
+            for (int i = 0; i < V; ++i) t[i] = to_f32(e[a * V + i]);
             if (col < cols) store_fp8<V>(row + col, t, by);
         }
     }
@@ -72,7 +63,7 @@ template <typename T, int V> struct QuantUnit {
 
 template <typename T, int V> __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p) {
     using U = QuantUnit<T, V>;
-    constexpr int N = QUANT_ROWS, HALF = V == 8 ? 16 : 32;  // lanes of a block
+    constexpr int N = QUANT_ROWS, BPU = V == 8 ? 2 : 1, NB = N * BPU;  // blocks of a unit, of a warp's turn
     const int lane = threadIdx.x & 31;
     const int units = (p.K + U::COLS - 1) / U::COLS;
     const long long jobs = (p.rows + N - 1) / N * units, step = (long long)gridDim.x * 8;
@@ -92,16 +83,26 @@ template <typename T, int V> __global__ void __launch_bounds__(256) quant_rows_k
         const long long row1 = job < jobs ? job / units * N : p.rows;
         const int unit1 = job < jobs ? (int)(job % units) : 0;
         fetch(next, row1, unit1);
-        float mine = 0.f;  // lane i of a block keeps row i's scale
+        // every lane learns the blocks' largest magnitudes, one lane for each block turns its own into the scale
+        const int mine = lane & (NB - 1), i = mine / BPU, block = unit * BPU + mine % BPU;
+        float amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float scale = fp8_scale(max_lanes<HALF>(now[i].amax()));
-            now[i].store(p.q + (row + i) * p.q_stride, unit, lane, row + i < p.rows ? p.K : 0, Fp8Scale(scale));
-            if ((lane & (HALF - 1)) == i) mine = scale;
+        for (int k = 0; k < N; ++k) {
+            const float m = now[k].amax();
+#pragma unroll
+            for (int b = 0; b < BPU; ++b) {
+                const float all = max_lanes<32>(BPU == 1 || (lane >> 4) == b ? m : 0.f);
+                if (mine == k * BPU + b) amax = all;
+            }
         }
-        const int i = lane & (HALF - 1), block = unit * (U::COLS / FP8_BLOCK) + lane / HALF;
-        if (i < N && row + i < p.rows && block * FP8_BLOCK < p.K)
-            p.scales[(row + i) * p.scale_row + (long long)block * p.scale_blk] = mine;
+        const float scale = fp8_scale(amax);
+        const Fp8Scale by(scale);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            now[k].store(p.q + (row + k) * p.q_stride, unit, lane, row + k < p.rows ? p.K : 0,
+                         by.from_lane(k * BPU + (BPU == 2 ? lane >> 4 : 0)));
+        if (lane < NB && row + i < p.rows && block * FP8_BLOCK < p.K)
+            p.scales[(row + i) * p.scale_row + (long long)block * p.scale_blk] = scale;
         if (job >= jobs) return;
         row = row1;
         unit = unit1;
@@ -151,7 +152,7 @@ template <typename T, int V> __global__ void __launch_bounds__(256) quant_blocks
             const int col = col0 + a * 32 * V + lane * V;
             float t[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) t[i] = -v[r][a * V + i];
+            for (int i = 0; i < V; ++i) t[i] = v[r][a * V + i];
             if (row < p.rows && col < p.K) store_fp8<V>(p.q + row * p.q_stride + col, t, by);
         }
     }
