@@ -609,7 +609,7 @@ template <typename K> long long resident_ctas(K kernel, int threads, int smem) {
 // =============================================================================================
 extern "C" {
 
-int qssm_version(void) { return 200; }
+int qssm_version(void) { return 210; }
 
 int qssm_tune_set(const char* name, int value) {
     if (name == nullptr) return QSSM_E_NULL;

@@ -79,10 +79,12 @@ def gated_scan_chunk(pa: torch.Tensor, px: torch.Tensor, pc1: torch.Tensor, pc2:
         y = torch.empty((B, L, D), dtype=out_dtype, device=pa.device)
         h_last = torch.empty((B, D), dtype=torch.float32, device=pa.device)
         try:
-            _lib.gated_scan_fwd(pa, px, pc1, pc2, pd, y, gate_dtype, h_in=None if state is None else state.h,
-                                h_last=h_last)
+            _lib.gated_scan_fwd(pa, px, pc1, pc2, pd, y, gate_dtype,
+                                h_in=None if state is None else state.h.contiguous(), h_last=h_last)
             return y, ScanState(h_last)
         except _lib.Unsupported:
             pass
     a, x, c, b = _gates(pa, px, pc1, pc2, pd, gate_dtype)
+    if state is not None:
+        state = ScanState(state.h.contiguous())
     return scan_chunk(x, a, b, c, state, out_dtype=out_dtype)

@@ -113,6 +113,7 @@ def test_c_entries_check_arguments_without_gpu():
         x, one, one, one, bias, one, M, N, K, xs, 1, M, 64, 1, 1, ys, out, 0, None, None)
     assert mm(M=0) == 0 and mm(N=0) == 0
     assert mm(M=-1) == -2 and mm(out=5) == -3 and mm(x=None) == -1
+    assert mm(K=0) == -2 and mm(M=2 ** 31) == -2
     assert mm(x=odd) == -4 and mm(xs=72) == -4 and mm(xs=48) == -4 and mm(ys=3) == -4
     norm = lambda rows=2, xd=2, rd=2, x=one, ys=8: lib.qssm_add_rmsnorm_fwd(  # noqa: E731
         x, one, one, one, one, None, rows, 8, 8, 8, ys, 8, 1e-5, xd, rd, 0, None)
@@ -445,6 +446,53 @@ def test_residual_norm_layouts_streams_and_refusals():
     h.add_(1)  # the backward needs h as it was
     with pytest.raises(RuntimeError, match="inplace"):
         y.sum().backward()
+
+
+@gpu
+def test_residual_norm_of_nothing_and_gradients_of_one_output():
+    w = torch.rand(8, device="cuda", requires_grad=True)
+    for shape, wt in (((0, 8), w), ((3, 0), torch.rand(0, device="cuda", requires_grad=True))):
+        x, r = (torch.zeros(shape, device="cuda", requires_grad=True) for _ in range(2))
+        y, h = add_rms_norm(x, r, wt)
+        (y.sum() + h.sum()).backward()
+        assert y.shape == h.shape == x.grad.shape == r.grad.shape == shape and (wt.grad == 0).all()
+    x = torch.randn(4, 8, device="cuda").to(BF16).requires_grad_()
+    r = torch.randn(4, 8, device="cuda", requires_grad=True)
+    y, h = add_rms_norm(x, r, w)
+    h.sum().backward()  # only the sum was used: ones to both, each in its own type
+    assert x.grad.dtype == BF16 and r.grad.dtype == F32 and (x.grad == 1).all() and (r.grad == 1).all()
+    y, h = add_rms_norm(x, r, w)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y.float().sum(), r, create_graph=True)
+    with torch.no_grad():
+        y, h = add_rms_norm(x, r, w)
+    assert not y.requires_grad and not h.requires_grad
+
+
+@gpu
+def test_calls_on_two_streams_at_once():
+    """Products of both kernels, norms and quantisation on two streams without an order between them."""
+    jobs = []
+    for M, N, K in ((3000, 2000, 700), (9, 3000, 2000)):
+        x, w, _ = operands(M, N, K)
+        src, res, one = torch.randn(M, K, device="cuda"), torch.randn(M, K, device="cuda"), torch.ones(K, device="cuda")
+
+        def job(x=x, w=w, src=src, res=res, one=one):
+            q, h = add_rms_norm_fp8(src, res, one)
+            return fp8.matmul_fp8(x, w), fp8.matmul_fp8(q, w), h, fp8.quantize_rows(src).values.view(torch.uint8)
+
+        jobs.append((job, job()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(jobs[i][0]())
+    torch.cuda.synchronize()
+    for (_, want), results in zip(jobs, got):
+        assert all(torch.equal(a, b) for r in results for a, b in zip(r, want))
+    _lib.check_device_status(synchronize=True)
 
 
 @gpu

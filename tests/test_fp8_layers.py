@@ -267,6 +267,9 @@ def test_gated_chunks_on_slices_match_separate_gates():
         # gates rounded to bf16 from approximations good to bf16: a step of 2^-8 here and there
         for g, w in ((y, want), (torch.cat([y1, y2], 1), want), (s.h, ws.h), (s2.h, ws.h)):
             assert rel(g, w) < 2 ** -7
+        strided = ScanState(s1.h.t().contiguous().t())  # a state in another layout
+        y3, s3 = gated_scan_chunk(*(t[:, 11:] for t in parts), strided)
+        assert torch.equal(y3, y2) and torch.equal(s3.h, s2.h)
 
 
 @gpu
