@@ -459,7 +459,7 @@ def _ordinal(first: torch.Tensor, *others) -> int:
     return index
 
 
-_current_device = torch.cuda.current_device
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _call(fn, name: str, index: int, args) -> None:
@@ -536,7 +536,7 @@ def quant_fp8(x, q, scales, blocks: bool) -> None:
            _DTYPE_CODE[x.dtype]))
 
 
-def matmul_fp8(x, x_scales, w, w_scales, bias, y) -> None:
+def matmul_fp8(x, x_pitch, x_scales, w, w_pitch, w_scales, bias, y) -> None:
     """y [M, N] = x [M, K] @ w [N, K]^T + bias on e4m3 operands whose rows start on 16-byte boundaries."""
     index = _ordinal(x, x_scales, w, w_scales, bias)
     if _lib is None:
@@ -544,13 +544,13 @@ def matmul_fp8(x, x_scales, w, w_scales, bias, y) -> None:
     e = _status_words.get(index) or _status_entry(index)
     if e[2].value != 0:
         _raise_status(e)
-    M, K = x.shape
+    M, N = y.shape
     xr, xb = x_scales.stride()
     wr, wb = w_scales.stride()
     bp, bcode = (None, 0) if bias is None else (bias.data_ptr(), _DTYPE_CODE[bias.dtype])
     _call(_lib.qssm_matmul_fp8, "qssm_matmul_fp8", index,
-          (x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), bp, y.data_ptr(), M, w.shape[0], K,
-           x.stride(0), xr, xb, w.stride(0), wr, wb, y.stride(0), _DTYPE_CODE[y.dtype], bcode, e[1]))
+          (x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), bp, y.data_ptr(), M, N, x.shape[1],
+           x_pitch, xr, xb, w_pitch, wr, wb, N, _DTYPE_CODE[y.dtype], bcode, e[1]))
 
 
 MAX_PEERS, PEER_SLOTS = 16, 4

@@ -42,8 +42,8 @@ class Fp8Rows:
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if values.dtype is not _E4M3 or scales.dtype is not torch.float32:
             raise TypeError(f"values must be float8_e4m3fn and scales float32; got {values.dtype} and {scales.dtype}")
-        *lead, K = values.shape
-        if [*lead, n_blocks(K)] != list(scales.shape):
+        shape, of = values.shape, scales.shape
+        if len(shape) < 1 or len(of) != len(shape) or shape[:-1] != of[:-1] or (shape[-1] + 127) // 128 != of[-1]:
             raise ValueError(f"scales {tuple(scales.shape)} are not one for each 128 of a row of {tuple(values.shape)}")
         self.values, self.scales = values, scales
 
@@ -84,7 +84,7 @@ class Fp8Weight:
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if values.dtype is not _E4M3 or scales.dtype is not torch.float32:
             raise TypeError(f"values must be float8_e4m3fn and scales float32; got {values.dtype} and {scales.dtype}")
-        if values.dim() != 2 or [n_blocks(n) for n in values.shape] != list(scales.shape):
+        if values.dim() != 2 or scales.shape != ((values.shape[0] + 127) // 128, (values.shape[1] + 127) // 128):
             raise ValueError(f"scales {tuple(scales.shape)} are not one for each 128 x 128 block of {tuple(values.shape)}")
         self.values, self.scales = values, scales
 
@@ -146,46 +146,49 @@ def quantize_weight(w: torch.Tensor) -> Fp8Weight:
     return q
 
 
-def _copyable(values: torch.Tensor) -> torch.Tensor:
-    """[rows, K] values as the product's copies can address them: a copy where a row or the base is not on a 16-byte
-    boundary or the last axis is strided."""
+def _copyable(values: torch.Tensor):
+    """[rows, K] values as the product's copies can address them, and their pitch: a copy where a row or the base is not
+    on a 16-byte boundary or the last axis is strided."""
     rows, K = values.shape
     pitch, step = values.stride()
     if (step == 1 or K <= 1) and pitch % 16 == 0 and pitch >= K and values.data_ptr() % 16 == 0:
-        return values
+        return values, pitch
     out = _values_like(rows, K, values.device)
     out.copy_(values)
-    return out
+    return out, out.stride(0)
 
 
 def matmul_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, *,
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x @ w.T + bias`` on quantised operands: ``[..., N]`` in ``out_dtype`` (bf16, fp16 or fp32)."""
-    xv, xs, wv, ws = x.values, x.scales, w.values, w.scales
+    xv, xs, wv = x.values, x.scales, w.values
     if not xv.is_cuda:
         raise RuntimeError("matmul_fp8 needs CUDA tensors; there is no CPU path")
     if out_dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be float32, float16 or bfloat16; got {out_dtype}")
     N, K = wv.shape
-    if xv.shape[-1] != K:
-        raise ValueError(f"x has {xv.shape[-1]} columns, the weight {K}")
+    *lead, k = xv.shape
+    if k != K:
+        raise ValueError(f"x has {k} columns, the weight {K}")
     if bias is not None:
         if bias.shape != (N,):
             raise ValueError(f"bias is {tuple(bias.shape)}, expected {(N,)}")
         if bias.dtype not in _FLOATS:
             raise TypeError(f"bias must be float32, float16 or bfloat16; got {bias.dtype}")
-        bias = bias.detach().contiguous()
-    lead = xv.shape[:-1]
-    if xv.dim() != 2:
-        rows = 1
-        for n in lead:
-            rows *= n
+        if bias.requires_grad or not bias.is_contiguous():
+            bias = bias.detach().contiguous()
+    rows = 1
+    for n in lead:
+        rows *= n
+    if len(lead) != 1:
         xv, xs = xv.reshape(rows, K), xs.reshape(rows, xs.shape[-1])
-    y = torch.empty_strided((xv.shape[0], N), (N, 1), dtype=out_dtype, device=xv.device)
+    y = torch.empty_strided((rows, N), (N, 1), dtype=out_dtype, device=xv.device)
     if K == 0:  # an empty sum
         y.copy_(bias) if bias is not None else y.zero_()
     else:
-        _lib.matmul_fp8(_copyable(xv), xs, _copyable(wv), ws, bias, y)
+        xv, x_pitch = _copyable(xv)
+        wv, w_pitch = _copyable(wv)
+        _lib.matmul_fp8(xv, x_pitch, xs, wv, w_pitch, w.scales, bias, y)
     return y if len(lead) == 1 else y.view(*lead, N)
 
 
