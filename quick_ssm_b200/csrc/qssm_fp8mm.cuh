@@ -7,9 +7,10 @@
 // while the tensor cores work on the next block in the other buffer.  Inner sums and the sum over blocks are fp32;
 // the result is rounded once.
 //
-// Roles: one thread issues the bulk copies (TMA, 128-byte swizzle, zero fill behind the last row and the last k), one
-// the products, the other warps own the sums.  Every wait on a barrier gives up after two seconds and reports
-// QSSM_S_TMA_TIMEOUT; the CTA then still waits for its own copies and products and frees its tensor memory.
+// Roles: a warp issues the bulk copies (TMA, 128-byte swizzle, zero fill behind the last row and the last k), others the
+// products and the copies of scales and bias, the rest own the sums.  Every wait on a barrier gives up after some
+// seconds and reports QSSM_S_TMA_TIMEOUT; the CTA then still waits for its own copies and products and frees its tensor
+// memory.
 #pragma once
 #include "qssm_elem.cuh"
 #include "qssm_tc.cuh"
@@ -50,9 +51,12 @@ __device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) { return make_
 // The product of a block of k is issued as two of 128 columns, each with two buffers of tensor memory of its own.  What
 // bounds the kernel is the way of a buffer from its product through both CTAs' sums back to the next product, a chain of
 // latencies (issue, commit, test, read back, arrival on the other SM, test; a branch alone is 40 cycles).  So each
-// buffer has an issuing warp of its own, the scales arrive on the same barrier as the tiles, and the sums' loop has no
-// other wait than the one for its product.  Results leave through shared memory and bulk stores of 32 rows x 128 bytes
-// per warp, so that the sums' registers are free for the next tile at once.
+// buffer has an issuing warp of its own, and warps of their own fetch the scales (by groups of four blocks) and the next
+// tile's bias ahead.  Results leave through shared memory and bulk stores of 32 rows x 128 bytes per warp, so that the
+// sums' registers are free for the next tile at once.
+//
+// 16384x20480x1024 390 us, 1.77 PFLOP/s (450 us under the power limit, 1.54 GHz); 16384x1024x4096 76 us.  One issuing
+// warp for all buffers: 438 us; tiles of 128 x 256 by single CTAs whose sums fetch their own scales: 835 us.
 // ---------------------------------------------------------------------------------------------
 constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;        // a pair's tile
 constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
@@ -321,7 +325,8 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
 // Few rows: the weight is the first operand.  Tiles of 128 columns of y x T rows (T = 16 to 128), lane = column, so
 // the weight's rows fill the tensor cores' 128 lanes however few rows there are, and k is cut over the S CTAs of a
 // cluster, whose sums are added in rank order through distributed shared memory (each CTA adds every S-th row).
-// Bound by latencies: a CTA sees few blocks of k, each a copy, a product and a read back.
+// Bound by latencies: a CTA sees few blocks of k, each a copy, a product and a read back.  1x20480x1024 7.2 us,
+// 64x1024x4096 7.4 us (the many-rows kernel 14.7 and 19.5).
 // ---------------------------------------------------------------------------------------------
 template <int T> struct Few {
     static constexpr int A = 128 * MM_TILE_K, STAGE = A + T * MM_TILE_K;
