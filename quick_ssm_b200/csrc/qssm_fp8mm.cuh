@@ -63,7 +63,8 @@ constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
 constexpr int MMR_WARPS = 8, MMR_COLS = 128;                   // warps that hold sums, columns of each
 constexpr int MMR_THREADS = 32 * MMR_WARPS + 256;              // warp 8 copies, 9 to 12 products, 13 scales, 14 bias
 // Scales in flight: slots of four blocks, a block being 128 of x and two of w.
-constexpr int MMR_SLOTS = 4, MMR_GROUP = 4, MMR_BLOCK = 576, MMR_SLOT = MMR_GROUP * MMR_BLOCK;
+constexpr int MMR_SLOTS = 4, MMR_GROUP = 4, MMR_BLOCK = 576, MMR_SLOT = MMR_GROUP * MMR_BLOCK,
+              MMR_RING = MMR_SLOTS * MMR_GROUP;
 constexpr int MMR_OUT = MMR_STAGES * MMR_STAGE, MMR_BIAS = MMR_OUT + MMR_WARPS * 8192,
               MMR_SCALES = MMR_BIAS + 2 * MMR_N * 4, MMR_BARS = MMR_SCALES + MMR_SLOTS * MMR_SLOT,
               MMR_SMEM = MMR_BARS + 512 + 1024;
@@ -99,11 +100,11 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 2); }  // empty: both halves
-        for (int b = 0; b < 4; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, MMR_WARPS); }
+        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, 2 * MMR_WARPS); }
         for (int f = 0; f < MMR_SLOTS; ++f) { mbar_init(scaled + 8 * f, 32); mbar_init(used + 8 * f, MMR_WARPS); }
         for (int i = 0; i < 2; ++i) { mbar_init(biased + 8 * i, 1); mbar_init(unbiased + 8 * i, MMR_WARPS); }
-        mbar_init(last, 4);
+        mbar_init(last, 2);
         fence_barrier_init();
     }
     if (warp == MMR_WARPS + 1) tmem_alloc<2>(smem_u32(const_cast<uint32_t*>(tmem_at)), 512);
@@ -122,7 +123,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
             const uint32_t full0 = cluster_addr(full, 0);
             uint32_t it = 0;
             for (int t = pair; ok && t < tiles; t += pairs) {
-                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N + (int)rank * 64;
+                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N + (int)rank * 128;
                 for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
                     const uint32_t s = it % MMR_STAGES, round = it / MMR_STAGES;
                     if (round > 0) ok = mbar_wait_limit(empty + 8 * s, (round - 1) & 1);
@@ -132,7 +133,6 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                         if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * MMR_STAGE);
                         tma_load_2d_pair(at, &p.x_map, bar, kb * MM_TILE_K, m0);
                         tma_load_2d_pair(at + MMR_A, &p.w_map, bar, kb * MM_TILE_K, n0);
-                        tma_load_2d_pair(at + MMR_A + MMR_A / 2, &p.w_map, bar, kb * MM_TILE_K, n0 + 128);
                     }
                 }
             }
@@ -140,16 +140,16 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
             const uint32_t left = it < (uint32_t)MMR_STAGES ? it : (uint32_t)MMR_STAGES;
             for (uint32_t i = it - left; ok && i < it; ++i) ok = mbar_wait_limit(empty + 8 * (i % MMR_STAGES), (i / MMR_STAGES) & 1);
             if (!ok) wait_ns(1000000);
-        } else if (warp <= MMR_WARPS + 4) {
+        } else if (warp <= MMR_WARPS + 2) {
             if (rank == 0) {  // warp 9 + b issues the products of buffer b: every second block's, of one half of the columns
-                constexpr uint32_t idesc = fp8_idesc(MMR_M, 128);
-                const uint32_t b = warp - (MMR_WARPS + 1), half = b & 1;
-                const uint32_t my_taken = taken + 8 * b, my_done = done + 8 * b, d = tmem + b * 128;
+                constexpr uint32_t idesc = fp8_idesc(MMR_M, MMR_N);
+                const uint32_t b = warp - (MMR_WARPS + 1);
+                const uint32_t my_taken = taken + 8 * b, my_done = done + 8 * b, d = tmem + b * 256;
                 uint32_t round = 0;
-                for (uint32_t it = b >> 1; it < total; it += 2, ++round) {
+                for (uint32_t it = b; it < total; it += 2, ++round) {
                     const uint32_t s = it % MMR_STAGES;
                     const uint64_t x = smem_operand(base + s * MMR_STAGE),
-                                   w = smem_operand(base + s * MMR_STAGE + MMR_A + half * (MMR_A / 2));
+                                   w = smem_operand(base + s * MMR_STAGE + MMR_A);
                     ok = mbar_wait_limit(full + 8 * s, (it / MMR_STAGES) & 1);
                     if (round > 0) ok &= mbar_wait_limit(my_taken, (round - 1) & 1);
                     if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -179,7 +179,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                     const uint32_t group = it / MMR_GROUP, f = group % MMR_SLOTS, round = group / MMR_SLOTS;
                     if (it % MMR_GROUP == 0 && round > 0) ok = mbar_wait_limit(used + 8 * f, (round - 1) & 1);
                     if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                    const uint32_t at = base + MMR_SCALES + f * MMR_SLOT + (it % MMR_GROUP) * MMR_BLOCK + lane * 4;
+                    const uint32_t at = base + MMR_SCALES + it % MMR_RING * MMR_BLOCK + lane * 4;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         copy_4(at + 128 * i, xs[i]);
@@ -211,10 +211,15 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
         regs_up<MMR_REGS_SUMS>();
         const int quarter = warp & 3, half = warp >> 2, col0 = half * MMR_COLS;
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
-        const uint32_t taken0 = cluster_addr(taken, 0) + 8 * half, my_done = done + 8 * half;
+        const uint32_t taken0 = cluster_addr(taken, 0), my_done = done;
         const float* my_x = reinterpret_cast<const float*>(smem + MMR_SCALES) + quarter * 32 + lane;
         const float* my_w = reinterpret_cast<const float*>(smem + MMR_SCALES) + 128 + half;
+        auto scales_here = [&](uint32_t i) {
+            return mbar_wait_limit(scaled + 8 * (i / MMR_GROUP % MMR_SLOTS), (i / MMR_RING) & 1);
+        };
         uint32_t it = 0, turn = 0;
+        if (total > 0) ok = scales_here(0);
+        float sx = my_x[0], sw = my_w[0];  // the next block's
         for (int t = pair; ok && t < tiles; t += pairs, ++turn) {
             const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + quarter * 32, n0 = (t / p.m_tiles) * MMR_N + col0;
             float2 acc[MMR_COLS / 2];
@@ -234,16 +239,14 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                 for (int j = 0; j < MMR_COLS / 2; ++j) acc[j] = make_float2(0.f, 0.f);
             }
             for (int kb = 0; ok && kb < p.n_kb; ++kb, ++it) {
-                const uint32_t b = it & 1, f = (it / MMR_GROUP) % MMR_SLOTS, d = at + b * 256;
-                if (it % MMR_GROUP == 0) ok = mbar_wait_limit(scaled + 8 * f, (it / (MMR_GROUP * MMR_SLOTS)) & 1);
-                const uint32_t where = f * (MMR_SLOT / 4) + (it % MMR_GROUP) * (MMR_BLOCK / 4);
-                const float factor = my_x[where] * my_w[where];  // scale of the row x scale of the weight's block
-                const float2 s = make_float2(factor, factor);
-                ok &= mbar_wait_limit(my_done + 16 * b, (it >> 1) & 1);
+                const uint32_t b = it & 1, d = at + b * 256, ni = it + 1;
+                ok &= mbar_wait_limit(my_done + 8 * b, (it >> 1) & 1);
                 tc_fence_after();
                 uint32_t r0[32], r1[32];
                 tmem_ld<32>(d, r0);
                 tmem_ld<32>(d + 32, r1);
+                const float factor = sx * sw;  // scale of the row x scale of the weight's block
+                const float2 s = make_float2(factor, factor);
                 tc_wait_ld(r0);
                 tc_landed(r1);
 #pragma unroll
@@ -252,14 +255,15 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
 #pragma unroll
                 for (int j = 0; j < 16; ++j) fma_pair(acc[16 + j], as_pair(r1[2 * j], r1[2 * j + 1]), s);
                 tmem_ld<32>(d + 96, r1);
+                // while those come: the next block's scales
+                if (ni % MMR_GROUP == 0 && ni < total) ok &= scales_here(ni);
+                sx = my_x[ni % MMR_RING * (MMR_BLOCK / 4)];
+                sw = my_w[ni % MMR_RING * (MMR_BLOCK / 4)];
                 tc_wait_ld(r0);
                 tc_landed(r1);
                 tc_fence_before();  // all read: the buffer may be written again
-                __syncwarp();
-                if (lane == 0 && ok) {
-                    mbar_arrive_cluster(taken0 + 16 * b);
-                    if (it % MMR_GROUP == MMR_GROUP - 1) mbar_arrive(used + 8 * f);
-                }
+                mbar_arrive_cluster_if(lane == 0 && ok, taken0 + 8 * b);
+                mbar_arrive_if(lane == 0 && ok && ni % MMR_GROUP == 0, used + 8 * (it / MMR_GROUP % MMR_SLOTS));
 #pragma unroll
                 for (int j = 0; j < 16; ++j) fma_pair(acc[32 + j], as_pair(r0[2 * j], r0[2 * j + 1]), s);
 #pragma unroll

@@ -66,6 +66,18 @@ __device__ __forceinline__ void copies_arrive(uint32_t bar) {
 }
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// The same arrivals by the lanes that `yes` names, without a branch around them.
+__device__ __forceinline__ void mbar_arrive_if(bool yes, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar),
+                 "r"((uint32_t)yes)
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster_if(bool yes, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar),
+                 "r"((uint32_t)yes)
+                 : "memory");
+}
+
 // ---- tensor memory ----------------------------------------------------------------------------
 // G = 1: one CTA; 2: both CTAs of a pair, each with a whole warp.
 template <int G> __device__ __forceinline__ void tmem_alloc(uint32_t where, uint32_t cols) {
