@@ -92,7 +92,7 @@ MatmulPlan plan_matmul(long long M, long long N, int n_kb, double ragged_us) {
     const long long sms = sm_count(), pairs = sms / 2;
     const long long big = ((M + MMR_M - 1) / MMR_M) * ((N + MMR_N - 1) / MMR_N);
     double best = 3.0 + (double)((big + pairs - 1) / pairs) * (0.47 * n_kb + 0.9 + ragged_us);
-    MatmulPlan plan{0, 1, 128, 128};
+    MatmulPlan plan{0, 1, 128, 64};
     const int T = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const double per_block = T == 16 ? 0.35 : T == 32 ? 0.4 : T == 64 ? 0.5 : 0.65;
     const long long tiles = ((N + 127) / 128) * ((M + T - 1) / T);

@@ -55,8 +55,11 @@ __device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) { return make_
 // tile's bias ahead.  Results leave through shared memory and bulk stores of 32 rows x 128 bytes per warp, so that the
 // sums' registers are free for the next tile at once.
 //
-// 16384x20480x1024 390 us, 1.77 PFLOP/s (450 us under the power limit, 1.54 GHz); 16384x1024x4096 76 us.  One issuing
-// warp for all buffers: 438 us; tiles of 128 x 256 by single CTAs whose sums fetch their own scales: 835 us.
+// 16384x20480x1024 374 us, 1.84 PFLOP/s (429 us under the power limit, 1.54 GHz); 16384x1024x4096 71 us;
+// 16384x8192x8192 1.1 ms.  The sums' loop has few branches for the same reason: the next block's scales are read in the
+// shadow of the second pair of reads, and the barriers are handed on by predicated arrivals.  One product of 256 columns
+// and one issuing warp per block: 391 us (450); one issuing warp for all buffers: 438 us; sixteen warps of 64 columns:
+// 426 us; tiles of 128 x 256 by single CTAs whose sums fetch their own scales: 835 us.
 // ---------------------------------------------------------------------------------------------
 constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;        // a pair's tile
 constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
@@ -100,11 +103,11 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, 2 * MMR_WARPS); }
+        for (int s = 0; s < MMR_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 2); }  // empty: both halves
+        for (int b = 0; b < 4; ++b) { mbar_init(done + 8 * b, 1); mbar_init(taken + 8 * b, MMR_WARPS); }
         for (int f = 0; f < MMR_SLOTS; ++f) { mbar_init(scaled + 8 * f, 32); mbar_init(used + 8 * f, MMR_WARPS); }
         for (int i = 0; i < 2; ++i) { mbar_init(biased + 8 * i, 1); mbar_init(unbiased + 8 * i, MMR_WARPS); }
-        mbar_init(last, 2);
+        mbar_init(last, 4);
         fence_barrier_init();
     }
     if (warp == MMR_WARPS + 1) tmem_alloc<2>(smem_u32(const_cast<uint32_t*>(tmem_at)), 512);
@@ -123,7 +126,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
             const uint32_t full0 = cluster_addr(full, 0);
             uint32_t it = 0;
             for (int t = pair; ok && t < tiles; t += pairs) {
-                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N + (int)rank * 128;
+                const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128, n0 = (t / p.m_tiles) * MMR_N + (int)rank * 64;
                 for (int kb = 0; kb < p.n_kb; ++kb, ++it) {
                     const uint32_t s = it % MMR_STAGES, round = it / MMR_STAGES;
                     if (round > 0) ok = mbar_wait_limit(empty + 8 * s, (round - 1) & 1);
@@ -133,6 +136,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                         if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * MMR_STAGE);
                         tma_load_2d_pair(at, &p.x_map, bar, kb * MM_TILE_K, m0);
                         tma_load_2d_pair(at + MMR_A, &p.w_map, bar, kb * MM_TILE_K, n0);
+                        tma_load_2d_pair(at + MMR_A + MMR_A / 2, &p.w_map, bar, kb * MM_TILE_K, n0 + 128);
                     }
                 }
             }
@@ -140,16 +144,16 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
             const uint32_t left = it < (uint32_t)MMR_STAGES ? it : (uint32_t)MMR_STAGES;
             for (uint32_t i = it - left; ok && i < it; ++i) ok = mbar_wait_limit(empty + 8 * (i % MMR_STAGES), (i / MMR_STAGES) & 1);
             if (!ok) wait_ns(1000000);
-        } else if (warp <= MMR_WARPS + 2) {
+        } else if (warp <= MMR_WARPS + 4) {
             if (rank == 0) {  // warp 9 + b issues the products of buffer b: every second block's, of one half of the columns
-                constexpr uint32_t idesc = fp8_idesc(MMR_M, MMR_N);
-                const uint32_t b = warp - (MMR_WARPS + 1);
-                const uint32_t my_taken = taken + 8 * b, my_done = done + 8 * b, d = tmem + b * 256;
+                constexpr uint32_t idesc = fp8_idesc(MMR_M, 128);
+                const uint32_t b = warp - (MMR_WARPS + 1), half = b & 1;
+                const uint32_t my_taken = taken + 8 * b, my_done = done + 8 * b, d = tmem + b * 128;
                 uint32_t round = 0;
-                for (uint32_t it = b; it < total; it += 2, ++round) {
+                for (uint32_t it = b >> 1; it < total; it += 2, ++round) {
                     const uint32_t s = it % MMR_STAGES;
                     const uint64_t x = smem_operand(base + s * MMR_STAGE),
-                                   w = smem_operand(base + s * MMR_STAGE + MMR_A);
+                                   w = smem_operand(base + s * MMR_STAGE + MMR_A + half * (MMR_A / 2));
                     ok = mbar_wait_limit(full + 8 * s, (it / MMR_STAGES) & 1);
                     if (round > 0) ok &= mbar_wait_limit(my_taken, (round - 1) & 1);
                     if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -211,7 +215,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
         regs_up<MMR_REGS_SUMS>();
         const int quarter = warp & 3, half = warp >> 2, col0 = half * MMR_COLS;
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + half * 128;
-        const uint32_t taken0 = cluster_addr(taken, 0), my_done = done;
+        const uint32_t taken0 = cluster_addr(taken, 0) + 8 * half, my_done = done + 8 * half;
         const float* my_x = reinterpret_cast<const float*>(smem + MMR_SCALES) + quarter * 32 + lane;
         const float* my_w = reinterpret_cast<const float*>(smem + MMR_SCALES) + 128 + half;
         auto scales_here = [&](uint32_t i) {
@@ -240,7 +244,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
             }
             for (int kb = 0; ok && kb < p.n_kb; ++kb, ++it) {
                 const uint32_t b = it & 1, d = at + b * 256, ni = it + 1;
-                ok &= mbar_wait_limit(my_done + 8 * b, (it >> 1) & 1);
+                ok &= mbar_wait_limit(my_done + 16 * b, (it >> 1) & 1);
                 tc_fence_after();
                 uint32_t r0[32], r1[32];
                 tmem_ld<32>(d, r0);
@@ -262,7 +266,7 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                 tc_wait_ld(r0);
                 tc_landed(r1);
                 tc_fence_before();  // all read: the buffer may be written again
-                mbar_arrive_cluster_if(lane == 0 && ok, taken0 + 8 * b);
+                mbar_arrive_cluster_if(lane == 0 && ok, taken0 + 16 * b);
                 mbar_arrive_if(lane == 0 && ok && ni % MMR_GROUP == 0, used + 8 * (it / MMR_GROUP % MMR_SLOTS));
 #pragma unroll
                 for (int j = 0; j < 16; ++j) fma_pair(acc[32 + j], as_pair(r0[2 * j], r0[2 * j + 1]), s);
