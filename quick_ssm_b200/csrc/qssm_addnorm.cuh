@@ -208,7 +208,22 @@ template <typename T, int V> struct Packed {
         }
     }
     __device__ __forceinline__ float operator[](int i) const { return to_f32(e[i]); }
+    __device__ __forceinline__ void take(Packed& to) { to = *this; }
 };
+// A unit on its way: as it lies in memory too, but for 16-bit elements that come one or two at a time.
+template <typename T, int V> struct SingleUnit : Singles<T, V, Unit<V>::EPT> {
+    using Base = Singles<T, V, Unit<V>::EPT>;
+    __device__ __forceinline__ void load(const T* row, int unit, int lane, int cols) {
+#pragma unroll
+        for (int a = 0; a < Unit<V>::ACC; ++a) {
+            const int col = Unit<V>::col(unit, a, lane);
+            Base::load(a, row + col, col < cols);
+        }
+    }
+    __device__ __forceinline__ void take(Packed<T, V>& to) { Base::take(to.e); }
+};
+template <typename T, int V>
+using Coming = typename std::conditional<V <= 2 && sizeof(T) == 2, SingleUnit<T, V <= 2 ? V : 1>, Packed<T, V>>::type;
 
 // WPR: warps per row.  NU: units of a row held in registers by each of its warps, 0 for rows that are longer.  R: rows at
 // a time.
@@ -229,26 +244,40 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
         for (int u = 0; u < N; ++u) load_weight<V>(p, u * WPR + wid, lane, w[u]);
     }
     // rows held in registers: the next ones are on their way while these are worked on
-    Packed<TX, V> x[R][N], x_next[R][N];
-    Packed<TR, V> res[R][N], res_next[R][N];
-    auto fetch = [&](Packed<TX, V> (&xi)[R][N], Packed<TR, V> (&ri)[R][N], long long row0) {
+    Packed<TX, V> x[R][N];
+    Packed<TR, V> res[R][N];
+    Coming<TX, V> x_next[R][N];
+    Coming<TR, V> res_next[R][N];
+    auto fetch = [&](long long row0) {
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             const long long row = row0 + k;
             const int cols = row < p.rows ? H : 0;
 #pragma unroll
             for (int u = 0; u < N; ++u) {
-                xi[k][u].load(static_cast<const TX*>(p.x) + row * p.x_stride, u * WPR + wid, lane, cols);
+                x_next[k][u].load(static_cast<const TX*>(p.x) + row * p.x_stride, u * WPR + wid, lane, cols);
                 if (p.res != nullptr)
-                    ri[k][u].load(static_cast<const TR*>(p.res) + row * p.res_stride, u * WPR + wid, lane, cols);
+                    res_next[k][u].load(static_cast<const TR*>(p.res) + row * p.res_stride, u * WPR + wid, lane, cols);
             }
         }
     };
+    auto take = [&]() {
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                x_next[k][u].take(x[k][u]);
+                if (p.res != nullptr) res_next[k][u].take(res[k][u]);
+            }
+    };
     const long long begin = ((long long)blockIdx.x * ROWS + warp / WPR) * R;
-    if constexpr (NU > 0) fetch(x, res, begin);
+    if constexpr (NU > 0) {
+        fetch(begin);
+        take();
+    }
     for (long long row0 = begin; row0 < p.rows; row0 += step) {
         if constexpr (NU > 0) {
-            fetch(x_next, res_next, row0 + step);
+            fetch(row0 + step);
             float h[R][N][EPT];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
@@ -284,13 +313,7 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
                 }
                 if constexpr (FP8) put_units_fp8<V, WPR>(p, row0 + k, wid, lane, h[k]);
             }
-#pragma unroll
-            for (int k = 0; k < R; ++k)
-#pragma unroll
-                for (int u = 0; u < N; ++u) {
-                    x[k][u] = x_next[k][u];
-                    res[k][u] = res_next[k][u];
-                }
+            take();
         } else {
             const TX* xr = static_cast<const TX*>(p.x) + row0 * p.x_stride;
             const TR* rr = static_cast<const TR*>(p.res) + row0 * p.res_stride;
@@ -352,13 +375,21 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
     }
     // 16-bit rows: the next ones are on their way while these are worked on (with fp32 three more rows of registers cost
     // more warps than that brings)
-    constexpr bool AHEAD = sizeof(TR) == 2 && NU > 0;
-    struct Rows {
+    constexpr bool AHEAD = sizeof(TR) == 2 && NU > 0 && V >= 4;
+    struct Held {
         Packed<TR, V> h[R][N], e[R][N];
         Packed<TX, V> g[R][N];
         float r[R];
     };
-    auto fetch = [&](Rows& to, long long row0) {
+    struct Fetched {
+        Coming<TR, V> h[R][N], e[R][N];
+        Coming<TX, V> g[R][N];
+        float r[R];
+    };
+    // (four 16-bit elements at a time: the same fields moved one by one, 139 us against 169 on 65536x1020)
+    constexpr bool SINGLES = (V <= 2 && (sizeof(TX) == 2 || sizeof(TR) == 2)) || (V == 4 && sizeof(TX) == 2 && sizeof(TR) == 2);
+    using Next = typename std::conditional<SINGLES, Fetched, Held>::type;
+    auto fetch = [&](auto& to, long long row0) {
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             const long long row = row0 + k;
@@ -372,13 +403,35 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
             }
         }
     };
+    auto take = [&](Held& to, Next& from) {
+        if constexpr (!SINGLES) to = from;
+        else {
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                to.r[k] = from.r[k];
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                    from.h[k][u].take(to.h[k][u]);
+                    from.g[k][u].take(to.g[k][u]);
+                    from.e[k][u].take(to.e[k][u]);
+                }
+            }
+        }
+    };
     const long long begin = ((long long)blockIdx.x * ROWS + warp / WPR) * R;
-    Rows now, next;
-    if constexpr (AHEAD) fetch(now, begin);
+    Held now;
+    Next next;
+    if constexpr (AHEAD && SINGLES) {
+        fetch(next, begin);
+        take(now, next);
+    } else if constexpr (AHEAD) fetch(now, begin);
     for (long long row0 = begin; row0 < p.rows; row0 += step) {
         if constexpr (NU > 0) {
             if constexpr (AHEAD) fetch(next, row0 + step);
-            else fetch(now, row0);
+            else if constexpr (SINGLES) {
+                fetch(next, row0);
+                take(now, next);
+            } else fetch(now, row0);
             auto& h = now.h;
             auto& e = now.e;
             auto& g = now.g;
@@ -418,7 +471,7 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
                         store_unit<TR, V>(static_cast<TR*>(p.dres) + row * p.dres_stride, u * WPR + wid, lane, cols, d);
                 }
             }
-            if constexpr (AHEAD) now = next;
+            if constexpr (AHEAD) take(now, next);
         } else {
             const TR* hr = static_cast<const TR*>(p.h) + row0 * p.h_stride;
             const TX* gr = static_cast<const TX*>(p.dy) + row0 * p.dy_stride;

@@ -139,7 +139,7 @@ int qssm_quant_fp8_rows(const void* x, void* q, float* scales, int64_t rows, int
                         int64_t q_stride, int64_t scale_stride_row, int64_t scale_stride_blk, int dtype, void* stream) {
     const int rc = quant_check(x, q, scales, rows, K, x_stride, q_stride, dtype);
     if (rc || rows == 0 || K == 0) return rc;
-    QuantParams p{x, static_cast<uint8_t*>(q), scales, rows, x_stride, q_stride, scale_stride_row, scale_stride_blk, (int)K};
+    QuantParams p{x, static_cast<uint8_t*>(q), scales, rows, x_stride, q_stride, scale_stride_row, scale_stride_blk, (int)K, fits(q, q_stride, 16, 1)};
     return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
         constexpr int VEC = 16 / sizeof(T);
@@ -162,13 +162,20 @@ int qssm_quant_fp8_blocks(const void* w, void* q, float* scales, int64_t N, int6
     const int rc = quant_check(w, q, scales, N, K, w_stride, q_stride, dtype);
     if (rc || N == 0 || K == 0) return rc;
     if (N > 128ll * 65535) return QSSM_E_SHAPE;
-    QuantParams p{w, static_cast<uint8_t*>(q), scales, N, w_stride, q_stride, scale_stride_row, scale_stride_blk, (int)K};
+    QuantParams p{w, static_cast<uint8_t*>(q), scales, N, w_stride, q_stride, scale_stride_row, scale_stride_blk, (int)K, fits(q, q_stride, 16, 1)};
     return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const bool vec = K % 4 == 0 && fits(w, w_stride, 4 * sizeof(T), sizeof(T)) && fits(q, q_stride, 4, 1);
         const dim3 grid((unsigned)((K + FP8_BLOCK - 1) / FP8_BLOCK), (unsigned)((N + FP8_BLOCK - 1) / FP8_BLOCK));
-        if (vec) quant_blocks_kernel<T, 4><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-        else quant_blocks_kernel<T, 1><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        constexpr int VEC = 16 / sizeof(T);
+        const bool vec = K % VEC == 0 && fits(w, w_stride, 16, sizeof(T)) && fits(q, q_stride, VEC, 1);
+        if constexpr (VEC == 8) {
+            if (vec) quant_blocks16_kernel<T, false><<<grid, 256, 0, s>>>(p);
+            else quant_blocks16_kernel<T, true><<<grid, 256, 0, s>>>(p);
+        } else {
+            if (vec) quant_blocks_kernel<T, 4><<<grid, 256, 0, s>>>(p);
+            else quant_blocks_kernel<T, 1><<<grid, 256, 0, s>>>(p);
+        }
         return (int)cudaGetLastError();
     });
 }

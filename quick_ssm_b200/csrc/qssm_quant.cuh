@@ -15,6 +15,7 @@ struct QuantParams {
     float* scales;
     long long rows, x_stride, q_stride, scale_row, scale_blk;
     int K;
+    bool q_words;  // rows of q start on 16-byte boundaries
 };
 
 constexpr int QUANT_ROWS = 4;  // rows whose unit a warp takes at a time
@@ -33,6 +34,7 @@ template <typename T, int V> struct QuantUnit {
             reinterpret_cast<W*>(e)[a] = w;
         }
     }
+    __device__ __forceinline__ void take(QuantUnit& to) { to = *this; }
     // the largest magnitude, NaN if there is one; 16-bit types two at a time
     __device__ __forceinline__ float amax() const {
         if constexpr (std::is_same<T, float>::value) {
@@ -61,6 +63,21 @@ template <typename T, int V> struct QuantUnit {
     }
 };
 
+// A unit on its way: as it lies in memory too, but for 16-bit elements that come one or two at a time.
+template <typename T, int V> struct SingleQuant : Singles<T, V, QuantUnit<T, V>::EPT> {
+    using Base = Singles<T, V, QuantUnit<T, V>::EPT>;
+    __device__ __forceinline__ void load(const T* row, int unit, int lane, int cols) {
+#pragma unroll
+        for (int a = 0; a < QuantUnit<T, V>::ACC; ++a) {
+            const int col = unit * QuantUnit<T, V>::COLS + a * 32 * V + lane * V;
+            Base::load(a, row + col, col < cols);
+        }
+    }
+    __device__ __forceinline__ void take(QuantUnit<T, V>& to) { Base::take(to.e); }
+};
+template <typename T, int V>
+using QuantComing = typename std::conditional<V <= 2 && sizeof(T) == 2, SingleQuant<T, V <= 2 ? V : 1>, QuantUnit<T, V>>::type;
+
 template <typename T, int V> __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantParams p) {
     using U = QuantUnit<T, V>;
     constexpr int N = QUANT_ROWS, BPU = V == 8 ? 2 : 1, NB = N * BPU;  // blocks of a unit, of a warp's turn
@@ -69,20 +86,26 @@ template <typename T, int V> __global__ void __launch_bounds__(256) quant_rows_k
     const long long jobs = (p.rows + N - 1) / N * units, step = (long long)gridDim.x * 8;
     long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (job >= jobs) return;
-    U now[N], next[N];
-    auto fetch = [&](U (&into)[N], long long row, int unit) {
+    U now[N];
+    QuantComing<T, V> next[N];
+    auto fetch = [&](long long row, int unit) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            into[i].load(static_cast<const T*>(p.x) + (row + i) * p.x_stride, unit, lane, row + i < p.rows ? p.K : 0);
+            next[i].load(static_cast<const T*>(p.x) + (row + i) * p.x_stride, unit, lane, row + i < p.rows ? p.K : 0);
+    };
+    auto take = [&]() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) next[i].take(now[i]);
     };
     long long row = job / units * N;
     int unit = (int)(job % units);
-    fetch(now, row, unit);
+    fetch(row, unit);
+    take();
     for (;;) {  // the next units are on their way while these are worked on
         job += step;
         const long long row1 = job < jobs ? job / units * N : p.rows;
         const int unit1 = job < jobs ? (int)(job % units) : 0;
-        fetch(next, row1, unit1);
+        fetch(row1, unit1);
         // every lane learns the blocks' largest magnitudes, one lane for each block turns its own into the scale
         const int mine = lane & (NB - 1), i = mine / BPU, block = unit * BPU + mine % BPU;
         float amax = 0.f;
@@ -106,8 +129,7 @@ template <typename T, int V> __global__ void __launch_bounds__(256) quant_rows_k
         if (job >= jobs) return;
         row = row1;
         unit = unit1;
-#pragma unroll
-        for (int k = 0; k < N; ++k) now[k] = next[k];
+        take();
     }
 }
 
@@ -155,6 +177,48 @@ template <typename T, int V> __global__ void __launch_bounds__(256) quant_blocks
             for (int i = 0; i < V; ++i) t[i] = v[r][a * V + i];
             if (row < p.rows && col < p.K) store_fp8<V>(p.q + row * p.q_stride + col, t, by);
         }
+    }
+    if (threadIdx.x == 0) p.scales[(long long)blockIdx.y * p.scale_row + (long long)blockIdx.x * p.scale_blk] = scale;
+}
+
+// Blocks of 16-bit weights: eight elements a lane and access, 16 lanes to a row, kept as they came.  ANY: rows start
+// anywhere.  65536x1024 bf16 48 us, 65536x1023 62; four (one) at a time 58 (205).
+template <typename T, bool ANY> __global__ void __launch_bounds__(256) quant_blocks16_kernel(const QuantParams p) {
+    constexpr int PER = 16, TIMES = FP8_BLOCK / PER;  // rows at a time
+    using U = QuantUnit<T, 8>;
+    __shared__ float red[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = threadIdx.x & 15, col0 = blockIdx.x * FP8_BLOCK;
+    const int cols = p.K - col0 < FP8_BLOCK ? p.K - col0 : FP8_BLOCK;
+    const long long row0 = (long long)blockIdx.y * FP8_BLOCK + (threadIdx.x >> 4);
+    U v[TIMES];
+    float amax = 0.f;
+#pragma unroll
+    for (int r = 0; r < TIMES; ++r) {
+        const long long row = row0 + PER * r;
+        const T* at = static_cast<const T*>(p.x) + row * p.x_stride + col0;
+        const int here = row < p.rows ? cols : 0;
+        if constexpr (ANY) load_any8(at + 8 * l, here - 8 * l, v[r].e);
+        else v[r].load(at, 0, l, here);
+    }
+#pragma unroll
+    for (int r = 0; r < TIMES; ++r) amax = max_nan(amax, v[r].amax());
+    amax = max_lanes<32>(amax);
+    if (lane == 0) red[warp] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = max_nan(amax, red[k]);
+    const float scale = fp8_scale(amax);
+    const Fp8Scale by(scale);
+#pragma unroll
+    for (int r = 0; r < TIMES; ++r) {
+        const long long row = row0 + PER * r;
+        const int left = (row < p.rows ? cols : 0) - 8 * l;
+        uint8_t* q = p.q + row * p.q_stride + col0 + 8 * l;
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = to_f32(v[r].e[i]);
+        if constexpr (ANY) store_fp8_part<8>(q, t, by, left, p.q_words);
+        else if (left > 0) store_fp8<8>(q, t, by);
     }
     if (threadIdx.x == 0) p.scales[(long long)blockIdx.y * p.scale_row + (long long)blockIdx.x * p.scale_blk] = scale;
 }

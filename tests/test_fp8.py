@@ -185,6 +185,28 @@ def test_quantisation_of_strided_and_nested_inputs():
     assert torch.equal(fp8.quantize_weight(base[0].t()).scales.cpu(), plain_quantize(base[0].t().cpu(), 128)[1])
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=ids)
+@pytest.mark.parametrize("K", [1, 7, 9, 130, 255])
+@pytest.mark.parametrize("blocks", [False, True], ids=["rows", "weight"])
+def test_quantisation_at_every_offset_leaves_the_neighbours_alone(K, blocks, dtype):
+    """Sources and values that start at each element of a 16-byte word, NaN around the source, marks around the values."""
+    rows, pitch = 131, K + 3
+    g = torch.Generator().manual_seed(K)
+    data = (torch.randn(rows, K, generator=g) * 3).to(dtype)
+    q, s = plain_quantize(data.float(), 128 if blocks else 1)
+    for off in range(8):
+        room = torch.full((off + rows * pitch + 16,), math.nan, dtype=dtype, device="cuda")
+        x = room[off:off + rows * pitch].view(rows, pitch)[:, :K]
+        x.copy_(data)
+        out = torch.full((off + rows * pitch + 16,), 0x55, dtype=torch.uint8, device="cuda")
+        values = out[off:off + rows * pitch].view(rows, pitch)
+        scales = torch.empty_like(s, device="cuda")
+        _lib.quant_fp8(x, values[:, :K], scales, blocks)
+        assert torch.equal(scales.cpu(), s) and torch.equal(values[:, :K].cpu(), q.view(torch.uint8))
+        assert (out[:off] == 0x55).all() and (values[:, K:] == 0x55).all() and (out[off + rows * pitch:] == 0x55).all()
+
+
 # ------------------------------------------------------------------------------------------------
 # the product
 # ------------------------------------------------------------------------------------------------
