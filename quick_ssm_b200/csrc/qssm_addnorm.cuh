@@ -31,6 +31,8 @@ constexpr int ADDNORM_WARPS = 8;      // warps per CTA
 constexpr int ADDNORM_HELD = 16;      // elements of a row that a lane holds in registers
 constexpr int ADDNORM_CTAS = 4;       // upper bound of CTAs per SM in the backward (sizes its scratch)
 
+constexpr int ADDNORM_HELD_DW = 72 * 1024;  // bytes of dw sums that a CTA holds, three CTAs on an SM
+
 struct AddNormParams {
     const void* x;
     const void* res;     // NULL: h is x
@@ -47,6 +49,7 @@ struct AddNormParams {
     long long rows, x_stride, res_stride, y_stride, h_stride, dy_stride, dh_stride, dx_stride, dres_stride;
     long long scale_row, scale_blk;
     int H, w_dtype, w_vec;
+    bool dw_held;        // backward, long rows: shared memory holds the CTA's dw sums
     float eps;
 };
 
@@ -350,13 +353,15 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_fwd_kernel(const A
 }
 
 // Backward.  Each warp keeps the dw sums of its columns: in registers over all its rows (NU > 0), added up over the
-// CTA's row groups in order at the end; for longer rows (eight warps each) in the CTA's part of the scratch.  What a row
-// brings stays packed as it came.
+// CTA's row groups in order at the end; for longer rows (eight warps each) in shared memory, or, where three CTAs on an SM
+// have no room for that, in the CTA's part of the scratch (4096x16384 bf16 205 us against 249 in the scratch, with an fp32
+// residual 346 against 392; with two CTAs on an SM shared memory is the slower one: 20480 columns 444 against 412).  What a
+// row brings stays packed as it came.
 template <typename TX, typename TR, int V, int WPR, int NU, int R>
 __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const AddNormParams p) {
     constexpr int EPT = Unit<V>::EPT, N = NU > 0 ? NU : 1;
     __shared__ float red[2][ADDNORM_WARPS];
-    extern __shared__ float dw_sum[];  // WPR < 8, NU > 0: H floats
+    extern __shared__ __align__(16) float dw_sum[];  // WPR < 8 or long rows: H floats
     int turn = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wid = warp % WPR;
     constexpr int ROWS = ADDNORM_WARPS / WPR;
@@ -370,8 +375,10 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
     for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int i = 0; i < EPT; ++i) dw[u][i] = 0.f;
+    // long rows: the sums lie in shared memory where that holds them, in the scratch otherwise
+    float* const sums = NU == 0 && p.dw_held ? dw_sum : part;
     if constexpr (NU == 0) {
-        for (int u = wid; u < units; u += WPR) store_unit<float, V>(part, u, lane, H, dw[0]);
+        for (int u = wid; u < units; u += WPR) store_unit<float, V>(sums, u, lane, H, dw[0]);
     }
     // 16-bit rows: the next ones are on their way while these are worked on (with fp32 three more rows of registers cost
     // more warps than that brings)
@@ -485,13 +492,13 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
                 load_unit<TR, V>(hr, u, lane, H, h);
                 load_unit<TX, V>(gr, u, lane, H, g);
                 load_weight<V>(p, u, lane, w);
-                load_unit<float, V>(part, u, lane, H, s);
+                load_unit<float, V>(sums, u, lane, H, s);
 #pragma unroll
                 for (int i = 0; i < EPT; ++i) {
                     dot = fmaf(h[i], g[i] * w[i], dot);
                     s[i] = fmaf(g[i] * r, h[i], s[i]);
                 }
-                store_unit<float, V>(part, u, lane, H, s);
+                store_unit<float, V>(sums, u, lane, H, s);
             }
             dot = sum_row<WPR>(dot, red, turn);
             const float k = dot * inv_h * r * r * r;
@@ -507,6 +514,15 @@ __global__ void __launch_bounds__(32 * ADDNORM_WARPS) addnorm_bwd_kernel(const A
                 for (int i = 0; i < EPT; ++i) e[i] += fmaf(-h[i], k, r * (w[i] * g[i]));
                 if (p.dx != nullptr) store_unit<TX, V>(dxr, u, lane, H, e);
                 if (p.dres != nullptr) store_unit<TR, V>(drr, u, lane, H, e);
+            }
+        }
+    }
+    if constexpr (NU == 0) {
+        if (p.dw_held) {
+            for (int u = wid; u < units; u += WPR) {
+                float s[EPT];
+                load_unit<float, V>(sums, u, lane, H, s);
+                store_unit<float, V>(part, u, lane, H, s);
             }
         }
     }

@@ -52,10 +52,19 @@ int qssm_add_rmsnorm_bwd(const void* h, const void* w, const void* dy, const voi
         return addnorm_variant<TX, TR>(V, rows, (int)H, [&](auto v, auto wpr, auto nu, auto at_once) -> int {
             constexpr int W = decltype(wpr)::value, NU = decltype(nu)::value, R = decltype(at_once)::value,
                           ROWS = ADDNORM_WARPS / W * R;
-            const long long need = (rows + ROWS - 1) / ROWS, most = (long long)ADDNORM_CTAS * sm_count();
+            p.dw_held = NU == 0 && H * 4 <= ADDNORM_HELD_DW;
+            const int smem = (W < ADDNORM_WARPS && NU > 0) || p.dw_held ? (int)H * 4 : 0;  // at most 16 KB but for long rows
+            const int room = 227 * 1024 / (smem + 1024), ctas = room < ADDNORM_CTAS ? room : ADDNORM_CTAS;  // of an SM
+            const long long need = (rows + ROWS - 1) / ROWS, most = (long long)ctas * sm_count();
             n_part = (int)(need < most ? need : most);
-            const int smem = W < ADDNORM_WARPS && NU > 0 ? (int)H * 4 : 0;  // at most 16 KB
-            addnorm_bwd_kernel<TX, TR, decltype(v)::value, W, NU, R><<<(unsigned)n_part, 32 * ADDNORM_WARPS, smem, stream>>>(p);
+            auto kernel = addnorm_bwd_kernel<TX, TR, decltype(v)::value, W, NU, R>;
+            if (NU == 0) {  // by itself the runtime may leave shared memory for fewer CTAs than fit
+                int e = p.dw_held ? ensure_smem(kernel, ADDNORM_HELD_DW) : 0;
+                if (e == 0)
+                    e = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, p.dw_held ? 100 : -1);
+                if (e) return e;
+            }
+            kernel<<<(unsigned)n_part, 32 * ADDNORM_WARPS, smem, stream>>>(p);
             return (int)cudaGetLastError();
         });
     });

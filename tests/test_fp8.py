@@ -380,6 +380,23 @@ def test_residual_norm_backward(shape, types):
 
 
 @gpu
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (BF16, F32)], ids=lambda t: "-".join(map(ids, t)))
+@pytest.mark.parametrize("shape", [(1300, 8200), (900, 10001), (700, 20480)], ids=str)
+def test_weight_gradient_of_long_rows_over_many_rows_per_cta(shape, types):
+    """Rows too long for registers, more of them than CTAs: the sums of dw that a CTA keeps in shared memory or scratch."""
+    (rows, H), (xd, rd) = shape, types
+    x, res, w, g = norm_inputs(rows, H, xd, rd)
+    dy = torch.randn(rows, H, generator=g).to(xd)
+    _, h, r = plain_norm(x, res, w, 1e-5)
+    terms = dy.double() * h.double() * r
+    dw, dw_mag = terms.sum(0), terms.abs().sum(0)
+    leaves = [t.cuda().requires_grad_() for t in (x, res, w)]
+    for _ in range(2):
+        grad, = torch.autograd.grad(add_rms_norm(*leaves)[0], leaves[2], dy.cuda())
+        assert ((grad.double().cpu() - dw).abs() <= (rows + H / 256 + 96) * U * dw_mag + 1e-30).all()
+
+
+@gpu
 def test_residual_norm_gradient_against_differences():
     """The kernel's gradient against differences of the 64-bit formula, with shared and broadcast inputs: one residual
     row for all, and x used as its own residual."""
