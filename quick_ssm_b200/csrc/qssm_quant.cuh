@@ -1,9 +1,9 @@
 // Quantisation to e4m3 with a scale for each 128 values of a row (activations) or each 128 x 128 block (weights).
 //
-// Bound by memory: one read of the source, one byte written per value.  Rows: a warp takes one unit of
-// four adjacent rows at a time (a unit is 256 columns in 16-byte accesses for 16-bit data, 128 otherwise), whose scales
-// lie side by side, with the next four on their way; a reduction over lanes per 128-column block.  Weights: a CTA takes one block, each warp 16 of its rows, and keeps it in registers
-// between the reduction and the output.
+// Bound by memory: one read of the source, one byte written per value.  Rows: a warp takes one unit of four adjacent rows at
+// a time (a unit is 256 columns in 16-byte accesses for 16-bit data, 128 otherwise), whose scales lie side by side, with the
+// next four on their way; a reduction over lanes per 128-column block.  Weights: a CTA takes one block and keeps it in
+// registers between the reduction and the output; of fp32 weights each warp has 16 rows, of 16-bit ones half a warp eight.
 #pragma once
 #include "qssm_elem.cuh"
 
