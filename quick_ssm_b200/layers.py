@@ -128,6 +128,8 @@ class SSMStack(nn.Module):
         first = self.layers[0]
         h, y = x, first._branch(rms_norm(x, first.pre_norm.weight, first.pre_norm.eps), scan_out_dtype)
         for layer in self.layers[1:]:
+            if h.dtype not in (y.dtype, torch.float32):  # as their sum would be promoted
+                h = h.float()
             u, h = add_rms_norm(y, h, layer.pre_norm.weight, layer.pre_norm.eps)
             y = layer._branch(u, scan_out_dtype)
         return y + h

@@ -86,6 +86,21 @@ def test_stack_trains_like_its_blocks_one_after_the_other():
 
 
 @gpu
+@pytest.mark.parametrize("x_dtype", [F32, BF16, torch.float16], ids=str)
+def test_stack_under_autocast_takes_the_types_that_its_blocks_take(x_dtype):
+    """bf16 branches on a residual stream of another type: promoted as the sequence's sums are."""
+    seq = torch.nn.Sequential(*(SSMFused(64, compute_dtype=BF16) for _ in range(3))).cuda()
+    stack = SSMStack(3, 64, compute_dtype=BF16).cuda()
+    stack.load_state_dict({f"layers.{k}": v for k, v in seq.state_dict().items()})
+    x = torch.randn(2, 9, 64, device="cuda").to(x_dtype)
+    with torch.autocast("cuda", dtype=BF16):
+        want, got = seq(x), stack(x)
+    assert got.dtype == want.dtype and got.shape == want.shape and torch.isfinite(got).all()
+    got.float().square().mean().backward()
+    assert all(torch.isfinite(p.grad).all() for p in stack.parameters())
+
+
+@gpu
 def test_residual_norm_captured_with_its_backward():
     """Forward and backward in one graph, replayed on new inputs, equal the eager passes bit for bit; two such graphs
     replayed in turn do not disturb each other."""
