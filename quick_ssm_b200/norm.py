@@ -82,9 +82,10 @@ def _check_add(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.
 
 
 def _room_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """An uninitialised contiguous tensor of t's shape (``empty_like`` takes half of ``empty``'s time on the host)."""
-    if t.dtype is dtype and t.is_contiguous():
-        return torch.empty_like(t)
+    """An uninitialised tensor of t's shape whose rows lie one behind the other (``empty_like`` takes half of ``empty``'s
+    time on the host).  Left to itself ``empty_like`` keeps t's strides, and those of axes of size 1 may be anything."""
+    if t.dtype is dtype:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
     return torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
@@ -113,7 +114,7 @@ class _AddRMSNormFunction(torch.autograd.Function):
         # autograd hands over gradients in the outputs' types and takes the inputs' own back
         xd, rd = dy.dtype, h.dtype
         dx = _room_like(h, xd) if need_x or rd is xd else None
-        dres = torch.empty_like(h) if rd is not xd and (need_r or dx is None) else None
+        dres = _room_like(h, rd) if rd is not xd and (need_r or dx is None) else None
         dw = torch.empty_like(w)
         _lib.add_rmsnorm_bwd(rows_2d(h), w, rows_2d(dy), None if dh is None else rows_2d(dh), rstd,
                              None if dx is None else rows_2d(dx), None if dres is None else rows_2d(dres), dw)

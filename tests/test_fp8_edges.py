@@ -1,0 +1,50 @@
+"""Edges of the residual norm and the 8-bit serving path: strides of axes of one, widths of types, sources at the end of
+their memory, weights that move between devices.  Bounds as derived in ``test_fp8.py``."""
+import pytest
+import torch
+
+from quick_ssm_b200.norm import _room_like, add_rms_norm, add_rms_norm_fp8
+
+from test_fp8 import BF16, F32, U, gpu, half_step, ids, plain_norm
+
+
+@pytest.mark.parametrize("shape,order", [((1, 8), (1, 0)), ((1, 1, 8), (2, 0, 1)), ((3, 1), (1, 0)), ((1, 5, 8), (1, 0, 2))], ids=str)
+def test_outputs_lie_row_by_row_whatever_the_strides_of_axes_of_one(shape, order):
+    """One token out of a transposed product has strides (1, 1): its outputs must not."""
+    t = torch.zeros([shape[i] for i in order]).permute([order.index(i) for i in range(len(shape))])
+    assert t.shape == shape
+    for dt in (F32, BF16):
+        room = _room_like(t, dt)
+        assert room.shape == shape and room.dtype == dt and room.stride() == torch.empty(shape).stride()
+
+
+@gpu
+@pytest.mark.parametrize("rd", [BF16, F32], ids=ids)
+@pytest.mark.parametrize("H", [8, 1024], ids=str)
+def test_one_token_out_of_a_transposed_product(H, rd):
+    """x, residual or both as a column transposed ([1, H] with strides (1, 1)): the results of the ordinary layout, whose
+    order of sums they need not share (the bounds of the tests above)."""
+    g = torch.Generator().manual_seed(H)
+    x, res, dy, dh = (torch.randn(1, H, generator=g).to(dt).cuda() for dt in (BF16, rd, BF16, rd))
+    w = (1 + torch.rand(H, generator=g)).cuda()
+    turned = lambda t: t.t().contiguous().t()  # noqa: E731
+    assert turned(x).stride() == (1, 1)
+    ref, _, r = plain_norm(x.cpu(), res.cpu(), w.cpu(), 1e-5)
+    lim = (half_step(BF16) + (H / 256 + 64) * U) * (1 + 2 ** -8) * ref.abs()
+    hd, gw = (x.float() + res.float()).to(rd).double().cpu(), dy.double().cpu() * w.double().cpu()
+    d = dh.double().cpu() + r * gw - hd * r ** 3 * (hd * gw).mean(-1, keepdim=True)
+    mag = dh.double().abs().cpu() + r * gw.abs() + hd.abs() * r ** 3 * (hd * gw).abs().mean(-1, keepdim=True)
+    c = (H / 256 + 64 + 3 * (H / 512 + 32)) * U
+    for a, b in ((turned(x), res), (x, turned(res)), (turned(x), turned(res)), (turned(x)[None], turned(res)[None])):
+        a, b = a.detach().requires_grad_(), b.detach().requires_grad_()
+        y, h = add_rms_norm(a, b, w)
+        torch.autograd.backward((y, h), (turned(dy).view_as(y), turned(dh).view_as(h)))
+        assert y.shape == a.shape and torch.equal(h.detach().view(1, H), (x.float() + res.float()).to(rd))
+        assert ((y.detach().view(1, H).double().cpu() - ref).abs() <= lim).all()
+        for leaf in (a, b):
+            assert ((leaf.grad.view(1, H).double().cpu() - d).abs() <= half_step(leaf.dtype) * (1 + 2 ** -8) * d.abs() + c * mag).all()
+        q, h8 = add_rms_norm_fp8(a.detach(), b.detach(), w)
+        assert q.shape == a.shape and torch.equal(h8, h.detach())
+        per = q.scales.view(1, -1).double().cpu().repeat_interleave(128, 1)[:, :H]
+        off = (q.dequantize().view(1, H).double().cpu() - ref).abs()
+        assert (off <= torch.maximum(2.0 ** -4 * ref.abs(), 2.0 ** -10 * per) * (1 + 2 ** -8) + (H / 256 + 64) * U * ref.abs()).all()
