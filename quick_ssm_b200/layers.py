@@ -143,7 +143,11 @@ class SSMFp8(nn.Module):
 
     ``forward(x, residual, state)`` takes the previous block's output and the residual stream apart (``residual=None``:
     x is the stream itself) and returns ``(out, residual, state)``; the stream behind this block is ``out + residual``.
-    ``state`` is a ``streaming.ScanState`` or None at the start of a sequence."""
+    ``state`` is a ``streaming.ScanState`` or None at the start of a sequence.
+
+    Gates are held in ``gate_dtype`` (the block's compute type, bfloat16 for a float32 one), projections, the scan's output
+    and ``out`` in ``act_dtype``: that type too, but float32 for float16 gates of a block whose weights are wider.  The block
+    holds these three in its weights' type, and what lies beyond float16's 65504 there is finite here as well."""
 
     def __init__(self, block: SSM, gate_dtype: Optional[torch.dtype] = None):
         super().__init__()
@@ -158,7 +162,9 @@ class SSMFp8(nn.Module):
             gate_dtype = block.compute_dtype if block.compute_dtype != torch.float32 else torch.bfloat16
         if gate_dtype not in (torch.bfloat16, torch.float16):
             raise TypeError(f"gates are bfloat16 or float16; got {gate_dtype}")
-        self.gate_dtype = gate_dtype
+        self.gate_dtype = self.act_dtype = gate_dtype
+        if gate_dtype == torch.float16 and block.out_proj.weight.dtype != torch.float16:
+            self.act_dtype = torch.float32
         with torch.no_grad():
             w_in = quantize_weight(torch.cat([m.weight for m in (block.A_proj, block.B_proj, block.C_proj_a,
                                                                  block.C_proj_b, block.D_proj)]))
@@ -185,9 +191,9 @@ class SSMFp8(nn.Module):
         from .norm import add_rms_norm_fp8
         from .streaming import gated_scan_chunk
         u, h = add_rms_norm_fp8(x, residual, self.norm_weight, self.eps)
-        p = matmul_fp8(u, self._weight("in"), self.in_bias, out_dtype=self.gate_dtype)
-        y, state = gated_scan_chunk(*p.split(self.state_size_dim, dim=-1), state)
-        out = matmul_fp8(quantize_rows(y), self._weight("out"), self.out_bias, out_dtype=self.gate_dtype)
+        p = matmul_fp8(u, self._weight("in"), self.in_bias, out_dtype=self.act_dtype)
+        y, state = gated_scan_chunk(*p.split(self.state_size_dim, dim=-1), state, gate_dtype=self.gate_dtype)
+        out = matmul_fp8(quantize_rows(y), self._weight("out"), self.out_bias, out_dtype=self.act_dtype)
         return out, h, state
 
 
@@ -212,7 +218,7 @@ class SSMStackFp8(nn.Module):
             raise ValueError("x must be [B, L, hidden]")
         y, h, after = x, None, []
         for layer, state in zip(self.layers, states):
-            # a residual stream in the branch's own type, or in fp32 under 16-bit branches
+            # a residual stream in the branch's own type, or in fp32
             y, h, state = layer(y, h, state)
             if h.dtype not in (y.dtype, torch.float32):
                 h = h.float()

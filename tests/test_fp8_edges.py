@@ -3,9 +3,12 @@ their memory, weights that move between devices.  Bounds as derived in ``test_fp
 import pytest
 import torch
 
+from quick_ssm_b200 import _lib
+from quick_ssm_b200.layers import SSM, SSMFp8, SSMStackFp8
 from quick_ssm_b200.norm import _room_like, add_rms_norm, add_rms_norm_fp8
 
-from test_fp8 import BF16, F32, U, gpu, half_step, ids, plain_norm
+from test_fp8 import BF16, F16, F32, U, gpu, half_step, ids, plain_norm
+from test_fp8_layers import blocks, plain_block, rel
 
 
 @pytest.mark.parametrize("shape,order", [((1, 8), (1, 0)), ((1, 1, 8), (2, 0, 1)), ((3, 1), (1, 0)), ((1, 5, 8), (1, 0, 2))], ids=str)
@@ -48,3 +51,46 @@ def test_one_token_out_of_a_transposed_product(H, rd):
         per = q.scales.view(1, -1).double().cpu().repeat_interleave(128, 1)[:, :H]
         off = (q.dequantize().view(1, H).double().cpu() - ref).abs()
         assert (off <= torch.maximum(2.0 ** -4 * ref.abs(), 2.0 ** -10 * per) * (1 + 2 ** -8) + (H / 256 + 64) * U * ref.abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("what", ["plain", "branch", "factors", "scan"])
+def test_serving_a_block_of_float16_gates_keeps_the_range_of_its_weights(what):
+    """The default compute type over fp32 weights: finite block outputs beyond 65504, a gate whose one factor is beyond it,
+    and a scan output beyond it.  The bound is that of the bf16 block in ``test_fp8_layers``: what is rounded to bf16 there
+    is rounded to fp16 or not at all here."""
+    block = blocks(1, 64, 2.0, compute=F16)[0]
+    with torch.no_grad():
+        if what == "branch":
+            block.out_proj.weight.mul_(1e6)
+        elif what == "factors":
+            block.C_proj_a.weight.mul_(1e6)
+            block.C_proj_b.weight.mul_(1e-6)
+        elif what == "scan":
+            block.B_proj.weight.mul_(1e4)
+            block.C_proj_a.weight.mul_(300)
+    served = SSMFp8(block)
+    torch.manual_seed(11)
+    x, r = torch.randn(3, 20, 64), torch.randn(3, 20, 64).mul(2)
+    out, h, state = served(x.cuda(), r.cuda())
+    want, want_h, want_s = plain_block(served, x, r, torch.zeros(3, 128, dtype=torch.float64))
+    if what == "branch":
+        assert want.abs().max() > 65504
+    assert served.gate_dtype == F16 and out.dtype == F32 and torch.equal(h.double().cpu(), want_h)
+    assert rel(out, want) < 0.03 and rel(state.h, want_s) < 0.03
+    y, _ = SSMStackFp8([block, block])(x.cuda().to(BF16))
+    assert y.dtype == BF16 and torch.isfinite(y).all()
+    _lib.check_device_status(synchronize=True)
+
+
+@gpu
+def test_serving_types_follow_the_block():
+    for weights, compute, gate, want in ((F32, F16, None, (F16, F32)), (F32, BF16, None, (BF16, BF16)), (F32, F32, None, (BF16, BF16)),
+                                         (F16, F16, None, (F16, F16)), (BF16, F16, None, (F16, F32)), (F32, F16, BF16, (BF16, BF16)),
+                                         (F32, BF16, F16, (F16, F32))):
+        served = SSMFp8(SSM(32, dtype=weights, compute_dtype=compute).cuda(), gate)
+        x = torch.randn(2, 5, 32, device="cuda").to(weights)
+        out, _, _ = served(x)
+        assert (served.gate_dtype, served.act_dtype) == want and out.dtype == want[1] and torch.isfinite(out).all()
+    with pytest.raises(TypeError, match="gates"):
+        SSMFp8(SSM(32).cuda(), F32)
