@@ -192,7 +192,9 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// The aligned forms want the whole warp at once: behind a branch that only some lanes took it is put together again first.
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

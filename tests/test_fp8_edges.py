@@ -1,13 +1,17 @@
 """Edges of the residual norm and the 8-bit serving path: strides of axes of one, widths of types, sources at the end of
 their memory, weights that move between devices.  Bounds as derived in ``test_fp8.py``."""
+import glob
+import os
+import re
+
 import pytest
 import torch
 
-from quick_ssm_b200 import _lib
+from quick_ssm_b200 import _lib, fp8
 from quick_ssm_b200.layers import SSM, SSMFp8, SSMStackFp8
 from quick_ssm_b200.norm import _room_like, add_rms_norm, add_rms_norm_fp8
 
-from test_fp8 import BF16, F16, F32, U, gpu, half_step, ids, plain_norm
+from test_fp8 import BF16, F16, F32, U, check_product, gpu, half_step, ids, operands, plain_norm
 from test_fp8_layers import blocks, plain_block, rel
 
 
@@ -94,3 +98,38 @@ def test_serving_types_follow_the_block():
         assert (served.gate_dtype, served.act_dtype) == want and out.dtype == want[1] and torch.isfinite(out).all()
     with pytest.raises(TypeError, match="gates"):
         SSMFp8(SSM(32).cuda(), F32)
+
+
+# ------------------------------------------------------------------------------------------------
+# barriers
+# ------------------------------------------------------------------------------------------------
+def barriers_without_a_whole_warp(pattern):
+    """Lines of inline PTX that match and have no ``__syncwarp();`` in the two lines in front of them."""
+    found, loose = 0, []
+    for path in sorted(glob.glob(os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc", "*.cu*"))):
+        with open(path) as f:
+            lines = f.read().splitlines()
+        for i, line in enumerate(lines):
+            if "asm" in line and re.search(pattern, line):
+                found += 1
+                if not any("__syncwarp();" in before for before in lines[max(0, i - 2):i]):
+                    loose.append(f"{os.path.basename(path)}:{i + 1}")
+    return found, loose
+
+
+def test_cluster_barriers_find_the_warp_whole():
+    """The aligned forms are undefined where only some lanes of a warp arrive together, and lanes that left a branch need
+    not be together again: sums are joined by the lanes whose column exists, and the barrier behind them keeps those sums alive."""
+    found, loose = barriers_without_a_whole_warp(r"barrier\.cluster\.arrive")
+    assert found == 1 and not loose
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(1, 1001, 4096), (16, 333, 8192), (40, 97, 4096), (64, 1005, 4096), (100, 300, 16384)], ids=str)
+def test_products_joined_over_a_cluster_with_columns_that_end_inside_a_warp(shape):
+    """k cut over clusters, N no multiple of 32, launches close behind each other: every one the same, and the formula's."""
+    x, w, bias = operands(*shape)
+    ys = [fp8.matmul_fp8(x, w, bias.cuda(), out_dtype=F32) for _ in range(40)]
+    check_product(ys[0], x, w, bias, str(shape))
+    assert all(torch.equal(y, ys[0]) for y in ys)
+    _lib.check_device_status(synchronize=True)
