@@ -118,6 +118,7 @@ template <int WPR> __device__ __forceinline__ float sum_row(float v, float (*red
     if constexpr (WPR > 1) {
         const int warp = threadIdx.x >> 5, group = warp / WPR;
         if ((threadIdx.x & 31) == 0) red[turn][warp] = v;
+        __syncwarp();  // the barrier wants the warp whole again
         if constexpr (WPR == ADDNORM_WARPS) __syncthreads();
         else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WPR) : "memory");
         v = 0.f;

@@ -124,6 +124,12 @@ def test_cluster_barriers_find_the_warp_whole():
     assert found == 1 and not loose
 
 
+def test_named_barriers_find_the_warp_whole():
+    """The same for the barrier of the warps that share a row, behind the store of one lane."""
+    found, loose = barriers_without_a_whole_warp(r'"bar\.sync')
+    assert found == 1 and not loose
+
+
 @gpu
 @pytest.mark.parametrize("shape", [(1, 1001, 4096), (16, 333, 8192), (40, 97, 4096), (64, 1005, 4096), (100, 300, 16384)], ids=str)
 def test_products_joined_over_a_cluster_with_columns_that_end_inside_a_warp(shape):
