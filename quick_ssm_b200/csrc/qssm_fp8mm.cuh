@@ -237,8 +237,9 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
                     acc[2 * j + 1] = make_float2(v.z, v.w);
                 }
                 __syncwarp();
-                if (lane == 0 && ok) mbar_arrive(unbiased + 8 * (turn & 1));
+                mbar_arrive_if(lane == 0 && ok, unbiased + 8 * (turn & 1));
             } else {
+                __syncwarp();  // one lane stored the tile before: the loop's loads are the whole warp's
 #pragma unroll
                 for (int j = 0; j < MMR_COLS / 2; ++j) acc[j] = make_float2(0.f, 0.f);
             }
@@ -449,6 +450,7 @@ __global__ void __launch_bounds__(Few<T>::THREADS, Few<T>::PER_SM) matmul_fp8_fe
             ok = mbar_wait_limit(scaled + 8 * f, (it / C::SLOTS) & 1);
             const float sw = scale[T];
             ok &= mbar_wait_limit(done + 8 * b, (it / C::BUFS) & 1);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;  // what follows is the whole warp's
             tc_fence_after();
             constexpr int L = C::ROWS < 32 ? C::ROWS : 32;  // rows read back at a time
 #pragma unroll

@@ -130,6 +130,22 @@ def test_named_barriers_find_the_warp_whole():
     assert found == 1 and not loose
 
 
+def test_tensor_memory_loads_find_the_warp_whole():
+    """Between a branch of one lane and the next aligned load of a product's kernels the warp is put together: from such a
+    branch on, the first of ``__syncwarp``, ``__all_sync`` and ``tmem_ld`` (around the loop as well) is no load."""
+    with open(os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc", "qssm_fp8mm.cuh")) as f:
+        text = f.read()
+    loops = [text[text.index("for (int t = pair; ok && t < tiles; t += pairs, ++turn) {\n            const int m0 = (t % p.m_tiles) * MMR_M + (int)rank * 128 + quarter"):text.index("if (lane == 0) tma_wait_all();")],
+             text[text.index("for (int j = 0; j < C::ROWS / 2; ++j) acc[j] = make_float2(0.f, 0.f);"):text.index("if (!ok && lane == 0 && p.status", text.index("matmul_fp8_few_kernel"))]]
+    for loop in loops:
+        marks = re.findall(r"if \(lane == 0|__syncwarp\(\)|__all_sync\(|tmem_ld<", loop)
+        assert "tmem_ld<" in marks and "if (lane == 0" in marks
+        for i, m in enumerate(marks):
+            if m == "if (lane == 0":
+                after = next(n for n in marks[i + 1:] + marks if n != "if (lane == 0")
+                assert after != "tmem_ld<", loop[:60]
+
+
 @gpu
 @pytest.mark.parametrize("shape", [(1, 1001, 4096), (16, 333, 8192), (40, 97, 4096), (64, 1005, 4096), (100, 300, 16384)], ids=str)
 def test_products_joined_over_a_cluster_with_columns_that_end_inside_a_warp(shape):
