@@ -102,9 +102,9 @@ class Fp8Weight:
         return (self.values.float() * per).to(dtype)
 
 
-def _values_like(rows: int, K: int, device) -> torch.Tensor:
-    """e4m3 [rows, K] whose rows start on 16-byte boundaries, as the product's copies need them."""
-    return torch.empty_strided((rows, K), ((K + 15) // 16 * 16, 1), dtype=_E4M3, device=device)
+def _values_like(rows: int, K: int, device, dtype: torch.dtype = _E4M3) -> torch.Tensor:
+    """e4m3 (or bytes) [rows, K] whose rows start on 16-byte boundaries, as the product's copies need them."""
+    return torch.empty_strided((rows, K), ((K + 15) // 16 * 16, 1), dtype=dtype, device=device)
 
 
 def rows_like(x2: torch.Tensor) -> Fp8Rows:
@@ -146,14 +146,14 @@ def quantize_weight(w: torch.Tensor) -> Fp8Weight:
     return q
 
 
-def _copyable(values: torch.Tensor):
+def copyable(values: torch.Tensor):
     """[rows, K] values as the product's copies can address them, and their pitch: a copy where a row or the base is not
     on a 16-byte boundary or the last axis is strided."""
     rows, K = values.shape
     pitch, step = values.stride()
     if (step == 1 or K <= 1) and pitch % 16 == 0 and pitch >= K and values.data_ptr() % 16 == 0:
         return values, pitch
-    out = _values_like(rows, K, values.device)
+    out = _values_like(rows, K, values.device, values.dtype)
     out.copy_(values)
     return out, out.stride(0)
 
@@ -186,8 +186,8 @@ def matmul_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, *,
     if K == 0:  # an empty sum
         y.copy_(bias) if bias is not None else y.zero_()
     else:
-        xv, x_pitch = _copyable(xv)
-        wv, w_pitch = _copyable(wv)
+        xv, x_pitch = copyable(xv)
+        wv, w_pitch = copyable(wv)
         _lib.matmul_fp8(xv, x_pitch, xs, wv, w_pitch, w.scales, bias, y)
     return y if len(lead) == 1 else y.view(*lead, N)
 

@@ -181,6 +181,21 @@ class SSMFp8(nn.Module):
         self.register_buffer(f"{name}_scales", w.scales)
         self.register_buffer(f"{name}_bias", bias)
 
+    def _space(self) -> None:
+        """Space the values' rows again where a move or a state dict has closed them up, once and not in every call."""
+        from .fp8 import copyable
+        for name in ("in_values", "out_values"):
+            setattr(self, name, copyable(getattr(self, name))[0])
+
+    def _apply(self, fn, recurse: bool = True):
+        super()._apply(fn, recurse)
+        self._space()
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._space()
+
     def _weight(self, name: str):
         from .fp8 import Fp8Weight
         return Fp8Weight(getattr(self, f"{name}_values").view(torch.float8_e4m3fn), getattr(self, f"{name}_scales"))

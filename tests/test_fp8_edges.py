@@ -1,5 +1,6 @@
 """Edges of the residual norm and the 8-bit serving path: strides of axes of one, widths of types, sources at the end of
 their memory, weights that move between devices.  Bounds as derived in ``test_fp8.py``."""
+import copy
 import glob
 import os
 import re
@@ -98,6 +99,50 @@ def test_serving_types_follow_the_block():
         assert (served.gate_dtype, served.act_dtype) == want and out.dtype == want[1] and torch.isfinite(out).all()
     with pytest.raises(TypeError, match="gates"):
         SSMFp8(SSM(32).cuda(), F32)
+
+
+# ------------------------------------------------------------------------------------------------
+# weights that move
+# ------------------------------------------------------------------------------------------------
+def spaced(block):
+    return all(getattr(block, k).stride(0) % 16 == 0 and getattr(block, k).stride(1) == 1 for k in ("in_values", "out_values"))
+
+
+def test_serving_weights_keep_their_spacing_without_a_gpu():
+    """A tensor with gaps between its rows loses them in a move; the block puts them back."""
+    block = SSMFp8.__new__(SSMFp8)
+    torch.nn.Module.__init__(block)
+    for name, (n, k) in (("in", (200, 40)), ("out", (40, 44))):
+        values = fp8._values_like(n, k, "cpu")
+        values.view(torch.uint8).copy_(torch.randint(0, 120, (n, k), dtype=torch.uint8))
+        block._keep(name, fp8.Fp8Weight(values, torch.rand(fp8.n_blocks(n), fp8.n_blocks(k))), torch.rand(n))
+    assert spaced(block)
+    before = {k: v.clone() for k, v in block.state_dict().items()}
+    assert before["in_values"].stride(0) == 40
+    at = block.in_values.data_ptr()
+    block.load_state_dict(before)
+    assert block.in_values.data_ptr() == at  # in place: a captured step still reads it
+    stack = torch.nn.Sequential(block)
+    for move in (lambda: stack._apply(lambda t: t.clone()), lambda: block.load_state_dict(before, assign=True)):
+        move()
+        assert spaced(block) and set(block.state_dict()) == set(before)
+        assert all(torch.equal(v, before[k]) for k, v in block.state_dict().items())
+
+
+@gpu
+def test_serving_weights_keep_their_spacing():
+    made = blocks(1, 72, 1.5)
+    x = torch.randn(2, 6, 72, device="cuda")
+    first = SSMFp8(made[0])
+    want = first(x)[0]
+    dense = {k: v.clone() for k, v in first.state_dict().items()}
+    moved, loaded = SSMFp8(made[0]).cpu().cuda(), SSMFp8(made[0])
+    loaded.load_state_dict(dense, assign=True)
+    for block in (first, moved, loaded, copy.deepcopy(first), copy.deepcopy(moved)):
+        assert spaced(block)
+        at = block.in_values.data_ptr()
+        assert torch.equal(block(x)[0], want) and block.in_values.data_ptr() == at
+        assert fp8.copyable(block.in_values)[0] is block.in_values
 
 
 # ------------------------------------------------------------------------------------------------
