@@ -358,6 +358,8 @@ int qssm_add_rmsnorm_bwd(const void* h, const void* w, const void* dy, const voi
  * rows  : a scale for each 128 values of a row (activations; the scan's output before the output projection).
  * blocks: a scale for each 128 x 128 block (weights), scales[bn*scale_stride_row + bk*scale_stride_blk].
  * A block that holds an infinity or a NaN gets an infinite or NaN scale and gives NaN wherever it is used.
+ * 16-bit weights on any boundary are read in words that may reach into the gaps between their rows, never in front of the
+ * first or behind the last element.
  */
 #define QSSM_FP8_BLOCK 128
 

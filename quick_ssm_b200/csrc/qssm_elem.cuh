@@ -95,8 +95,8 @@ template <typename T, int V, int N> struct Singles {
 };
 
 // Eight 16-bit elements from any element's address on, in 16-byte accesses: an aligned word and the one behind it, moved
-// into place in registers.  A word that holds one of the `left` elements is read whole (a word never crosses a page); zeros
-// stand for what lies behind them.
+// into place in registers.  A word that holds one of the `left` elements is read whole: it reaches up to seven elements over
+// their ends (`words_inside` says where it may).  Zeros stand for what lies behind them.
 template <typename T> __device__ __forceinline__ void load_any8(const T* p, int left, T (&out)[8]) {
     const int s = (int)(reinterpret_cast<uintptr_t>(p) >> 1) & 7;
     const uint4* at = reinterpret_cast<const uint4*>(p - s);
@@ -117,6 +117,15 @@ template <typename T> __device__ __forceinline__ void load_any8(const T* p, int 
 #pragma unroll
     for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(out)[i] = a[i];
 }
+// The same one by one.
+template <typename T> __device__ __forceinline__ void load_each8(const T* p, int left, T (&out)[8]) {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t*>(out)[i] = i < left ? e[i] : (uint16_t)0;
+}
+// Do the words around the elements from `first` to `last` of a source (counted from its first one) lie between the first and
+// the last of its `all` elements, gaps between rows included?
+__device__ __forceinline__ bool words_inside(long long first, long long last, long long all) { return first >= 7 && last + 7 <= all; }
 
 __device__ __forceinline__ float sum_warp(float v) {
 #pragma unroll

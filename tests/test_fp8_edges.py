@@ -4,6 +4,7 @@ import copy
 import glob
 import os
 import re
+import subprocess
 
 import pytest
 import torch
@@ -143,6 +144,71 @@ def test_serving_weights_keep_their_spacing():
         at = block.in_values.data_ptr()
         assert torch.equal(block(x)[0], want) and block.in_values.data_ptr() == at
         assert fp8.copyable(block.in_values)[0] is block.in_values
+
+
+# ------------------------------------------------------------------------------------------------
+# sources at the end of their memory
+# ------------------------------------------------------------------------------------------------
+HOST_SIDE = r"""
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+#define __device__
+#define __forceinline__ inline
+static uintptr_t from, upto;
+static long outside = 0;
+static void seen(const void* p, size_t n) { if ((uintptr_t)p < from || (uintptr_t)p + n > upto) ++outside; }
+struct uint4 {  // what is read is read through its copies
+    uint32_t x, y, z, w;
+    uint4() : x(0), y(0), z(0), w(0) {}
+    uint4(const uint4& o) { seen(&o, 16); memcpy(this, &o, 16); }
+    uint4& operator=(const uint4& o) { seen(&o, 16); memcpy(this, &o, 16); return *this; }
+};
+static uint32_t __funnelshift_r(uint32_t lo, uint32_t hi, uint32_t by) { return (uint32_t)((((uint64_t)hi << 32) | lo) >> (by & 31)); }
+%s
+int main() {
+    alignas(16) static uint16_t room[8192];
+    long wrong = 0, by_words = 0, by_each = 0;
+    for (int off = 0; off < 8; ++off)
+        for (int rows = 1; rows < 140; rows += rows < 4 ? 1 : 126)
+            for (int K = 1; K < 300; K += K < 20 ? 1 : 13)
+                for (int gap = -1; gap < 4; ++gap) {
+                    const long long stride = gap < 0 ? 0 : K + gap, all = (rows - 1) * stride + K;
+                    if (off + all + 64 > 8192) continue;
+                    for (int i = 0; i < 8192; ++i) room[i] = (uint16_t)(i * 7 + 1);
+                    const uint16_t* x = room + 32 + off;
+                    from = (uintptr_t)x; upto = (uintptr_t)(x + all);
+                    for (long long top = 0; top < rows; top += 128)
+                        for (int col0 = 0; col0 < K; col0 += 128) {  // as the kernel's blocks of 128 x 128
+                            const int cols = K - col0 < 128 ? K - col0 : 128;
+                            const long long bottom = top + 128 < rows ? top + 128 : rows;
+                            const bool words = words_inside(top * stride + col0, (bottom - 1) * stride + col0 + cols, all);
+                            ++(words ? by_words : by_each);
+                            for (long long row = top; row < bottom; ++row)
+                                for (int l = 0; l < 16; ++l) {
+                                    uint16_t out[8];
+                                    const uint16_t* at = x + row * stride + col0 + 8 * l;
+                                    if (words) load_any8<uint16_t>(at, cols - 8 * l, out);
+                                    else load_each8<uint16_t>(at, cols - 8 * l, out);
+                                    for (int i = 0; i < 8; ++i) wrong += out[i] != (8 * l + i < cols ? at[i] : 0);
+                                }
+                        }
+                }
+    printf("%%ld %%ld %%d", wrong, outside, by_words > 100 && by_each > 100);
+}
+"""
+
+
+def test_reads_of_sources_on_any_boundary_stay_in_the_source(tmp_path):
+    """The device functions, compiled for the host, over blocks of sources at every offset in a word: right elements, and no
+    16-byte word that reaches over the source's first or last element."""
+    with open(os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc", "qssm_elem.cuh")) as f:
+        text = f.read()
+    functions = text[text.index("template <typename T> __device__ __forceinline__ void load_any8"):text.index("__device__ __forceinline__ float sum_warp(")]
+    src, exe = tmp_path / "any8.cpp", tmp_path / "any8"
+    src.write_text(HOST_SIDE % functions)
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fno-strict-aliasing", "-o", str(exe), str(src)])
+    assert subprocess.check_output([str(exe)], text=True).split() == ["0", "0", "1"]
 
 
 # ------------------------------------------------------------------------------------------------
