@@ -88,12 +88,16 @@ class SSMFused(SSM):
             return super().forward(x, block_l=block_l, checkpoint=checkpoint, tile_b=tile_b, tile_d=tile_d,
                                    backend=backend, scan_out_dtype=scan_out_dtype)
         skip = x if self.use_residual else 0
-        if self.use_norm:  # the normalisation kernels on the layer's own weight
-            from .norm import rms_norm
-            u = rms_norm(x, self.pre_norm.weight, self.pre_norm.eps)
-        else:
-            u = x
-        return self._branch(u, scan_out_dtype) + skip
+        return self._branch(self._normed(x) if self.use_norm else x, scan_out_dtype) + skip
+
+    def _normed(self, x: torch.Tensor) -> torch.Tensor:
+        """The normalisation kernels on the layer's own weight.  They keep x's type; the plain norm's product promotes x to
+        the weight's, which the projections ask for unless autocast chooses their type."""
+        from .norm import rms_norm
+        w = self.pre_norm.weight
+        if x.dtype != w.dtype and not torch.is_autocast_enabled("cuda"):
+            x = x.to(torch.promote_types(x.dtype, w.dtype))
+        return rms_norm(x, w, self.pre_norm.eps)
 
     def _branch(self, u: torch.Tensor, scan_out_dtype: Optional[torch.dtype]) -> torch.Tensor:
         """The block behind its pre-norm and in front of its residual."""
@@ -108,8 +112,8 @@ class SSMFused(SSM):
 class SSMStack(nn.Module):
     """``n_layers`` residual SSM blocks, the same function as ``nn.Sequential`` of ``SSM`` with the same weights.
     The residual stream and the blocks' outputs are kept apart between two blocks, so that the residual's addition and
-    the next block's norm are one kernel per direction (``norm.add_rms_norm``).  ``layers`` holds the blocks; a state
-    dict of such a ``Sequential`` loads with its keys prefixed by ``layers.``."""
+    the next block's norm are one kernel per direction (``norm.add_rms_norm``); on the CPU and in float64 the blocks run one after the other.  ``layers`` holds the blocks; a state dict of such a ``Sequential`` loads with
+    its keys prefixed by ``layers.``.  Hooks are called on the projections, not on the blocks and their norms."""
 
     def __init__(self, n_layers: int, hidden_size: int, state_size_mult: float = 1.0, eps: float = 1e-5,
                  dtype: torch.dtype = torch.float32, device: Optional[torch.device] = None,
@@ -120,13 +124,14 @@ class SSMStack(nn.Module):
 
     def forward(self, x: torch.Tensor, *, backend: str = "auto",
                 scan_out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-        if backend == "torch" or x.device.type != "cuda" or not self.layers:
+        from .norm import FLOATS, add_rms_norm
+        if (backend == "torch" or x.device.type != "cuda" or not self.layers or x.dtype not in FLOATS
+                or self.layers[0].out_proj.weight.dtype not in FLOATS):
             for layer in self.layers:
                 x = layer(x, backend=backend, scan_out_dtype=scan_out_dtype)
             return x
-        from .norm import add_rms_norm, rms_norm
         first = self.layers[0]
-        h, y = x, first._branch(rms_norm(x, first.pre_norm.weight, first.pre_norm.eps), scan_out_dtype)
+        h, y = x, first._branch(first._normed(x), scan_out_dtype)
         for layer in self.layers[1:]:
             if h.dtype not in (y.dtype, torch.float32):  # as their sum would be promoted
                 h = h.float()

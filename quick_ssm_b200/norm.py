@@ -63,14 +63,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.
     return _RMSNormFunction.apply(x, weight, eps)
 
 
-_FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
+FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
 
 
 def _check_add(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, name: str) -> None:
     if not x.is_cuda:
         raise RuntimeError(f"{name} needs CUDA tensors; there is no CPU path")
     dt, shape = x.dtype, x.shape
-    if dt not in _FLOATS or weight.dtype not in _FLOATS:
+    if dt not in FLOATS or weight.dtype not in FLOATS:
         raise TypeError(f"{name} takes float32, float16 and bfloat16; got {dt} with a weight in {weight.dtype}")
     if len(shape) < 1 or weight.shape != shape[-1:]:
         raise ValueError("weight must have the size of the last axis of x")

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from quick_ssm_b200 import _lib, fp8
-from quick_ssm_b200.layers import SSM, SSMFp8, SSMStackFp8
+from quick_ssm_b200.layers import SSM, SSMFp8, SSMFused, SSMStack, SSMStackFp8
 from quick_ssm_b200.norm import _room_like, add_rms_norm, add_rms_norm_fp8
 
 from test_fp8 import BF16, F16, F32, U, check_product, gpu, half_step, ids, operands, plain_norm
@@ -100,6 +100,47 @@ def test_serving_types_follow_the_block():
         assert (served.gate_dtype, served.act_dtype) == want and out.dtype == want[1] and torch.isfinite(out).all()
     with pytest.raises(TypeError, match="gates"):
         SSMFp8(SSM(32).cuda(), F32)
+
+
+# ------------------------------------------------------------------------------------------------
+# types and arguments of the training blocks
+# ------------------------------------------------------------------------------------------------
+F64 = torch.float64
+
+
+@gpu
+@pytest.mark.parametrize("weights,xd", [(F32, F32), (F32, BF16), (F32, F16), (F64, F64), (F64, F32), (F64, BF16)], ids=ids)
+def test_stack_takes_the_types_that_its_blocks_take(weights, xd):
+    """Without autocast the plain blocks promote x to the weights' type.  The fused blocks and the stack do as well: the result
+    and the gradients of the plain blocks on x promoted beforehand, 1e-5 of the largest value per block and direction
+    (the order of fp32 sums).  x's gradient comes from two uses of x, the residual and the norm: autograd rounds each to x's
+    type and then their sum, three half steps of three magnitudes."""
+    seq = torch.nn.Sequential(*(SSM(64, 2.0, dtype=weights, compute_dtype=F32) for _ in range(3))).cuda()
+    fused = torch.nn.Sequential(*(SSMFused(64, 2.0, dtype=weights, compute_dtype=F32) for _ in range(3))).cuda()
+    stack = SSMStack(3, 64, 2.0, dtype=weights, compute_dtype=F32).cuda()
+    fused.load_state_dict(seq.state_dict())
+    stack.load_state_dict({f"layers.{k}": v for k, v in seq.state_dict().items()})
+    x = torch.randn(2, 9, 64, device="cuda").to(xd)
+    dy = torch.randn(2, 9, 64, device="cuda").to(weights)
+    x0 = x.clone().to(weights).requires_grad_()
+    first = seq[0](x0)
+    first.retain_grad()  # what the residual passes on
+    want = seq[2](seq[1](first))
+    want.backward(dy)
+    skip, total = first.grad.double(), x0.grad.double()
+    rounded = half_step(xd) * (1 + 2 ** -8) * (skip.abs() + (total - skip).abs() + total.abs())
+    assert seq(x).dtype == want.dtype
+    lim = lambda w: 6e-5 * w.abs().max()  # noqa: E731
+    for model, layers in ((fused, fused), (stack, stack.layers)):
+        xi = x.clone().requires_grad_()
+        got = model(xi)
+        got.backward(dy)
+        assert got.dtype == want.dtype and (got - want).abs().max() <= lim(want)
+        assert xi.grad.dtype == xd
+        assert ((xi.grad.double() - total).abs() <= lim(total) + rounded).all()
+        for p, q in zip(layers.parameters(), seq.parameters()):
+            assert (p.grad - q.grad).abs().max() <= lim(q.grad)
+    _lib.check_device_status(synchronize=True)
 
 
 # ------------------------------------------------------------------------------------------------
