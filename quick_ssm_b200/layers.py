@@ -112,7 +112,8 @@ class SSMFused(SSM):
 class SSMStack(nn.Module):
     """``n_layers`` residual SSM blocks, the same function as ``nn.Sequential`` of ``SSM`` with the same weights.
     The residual stream and the blocks' outputs are kept apart between two blocks, so that the residual's addition and
-    the next block's norm are one kernel per direction (``norm.add_rms_norm``); on the CPU and in float64 the blocks run one after the other.  ``layers`` holds the blocks; a state dict of such a ``Sequential`` loads with
+    the next block's norm are one kernel per direction (``norm.add_rms_norm``); on the CPU, without ``checkpoint`` and in
+    float64 the blocks run one after the other.  ``layers`` holds the blocks; a state dict of such a ``Sequential`` loads with
     its keys prefixed by ``layers.``.  Hooks are called on the projections, not on the blocks and their norms."""
 
     def __init__(self, n_layers: int, hidden_size: int, state_size_mult: float = 1.0, eps: float = 1e-5,
@@ -122,13 +123,15 @@ class SSMStack(nn.Module):
         self.layers = nn.ModuleList(SSMFused(hidden_size, state_size_mult, eps, dtype, device, compute_dtype)
                                     for _ in range(n_layers))
 
-    def forward(self, x: torch.Tensor, *, backend: str = "auto",
+    def forward(self, x: torch.Tensor, *, block_l: int = 256, checkpoint: bool = True,
+                tile_b: Optional[int] = None, tile_d: Optional[int] = None, backend: str = "auto",
                 scan_out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         from .norm import FLOATS, add_rms_norm
-        if (backend == "torch" or x.device.type != "cuda" or not self.layers or x.dtype not in FLOATS
+        if (backend == "torch" or x.device.type != "cuda" or not checkpoint or not self.layers or x.dtype not in FLOATS
                 or self.layers[0].out_proj.weight.dtype not in FLOATS):
             for layer in self.layers:
-                x = layer(x, backend=backend, scan_out_dtype=scan_out_dtype)
+                x = layer(x, block_l=block_l, checkpoint=checkpoint, tile_b=tile_b, tile_d=tile_d, backend=backend,
+                          scan_out_dtype=scan_out_dtype)
             return x
         first = self.layers[0]
         h, y = x, first._branch(first._normed(x), scan_out_dtype)

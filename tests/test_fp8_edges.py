@@ -143,6 +143,20 @@ def test_stack_takes_the_types_that_its_blocks_take(weights, xd):
     _lib.check_device_status(synchronize=True)
 
 
+@gpu
+def test_stack_takes_the_arguments_that_its_blocks_take():
+    stack = SSMStack(2, 32, compute_dtype=F32).cuda()
+    x = torch.randn(2, 40, 32, device="cuda")
+    want = stack(x)
+    for kw in (dict(block_l=16, tile_b=1, tile_d=8), dict(checkpoint=False), dict(backend="torch"), dict(scan_out_dtype=F32)):
+        seq = x
+        for layer in stack.layers:
+            seq = layer(seq, **kw)
+        got = stack(x, **kw)
+        # fp32 sums in another order, as above
+        assert (got - seq).abs().max() <= 4e-5 * seq.abs().max() and (got - want).abs().max() <= 4e-5 * want.abs().max()
+
+
 # ------------------------------------------------------------------------------------------------
 # weights that move
 # ------------------------------------------------------------------------------------------------
