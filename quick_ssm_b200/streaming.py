@@ -55,7 +55,7 @@ def scan_chunk(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: Optional[to
     k_out = _kernel_out_dtype(xs.dtype, out_dtype)
     y = torch.empty((B, L, D), dtype=k_out, device=x.device)
     h_last = torch.empty((B, D), dtype=torch.float32, device=x.device)
-    _lib.scan_fwd(xs, as_, bs, cs, y, h_in=None if state is None else state.h, h_last=h_last)
+    _lib.scan_fwd(xs, as_, bs, cs, y, h_in=None if state is None else state.h.contiguous(), h_last=h_last)
     return (y if k_out == out_dtype else y.to(out_dtype)), ScanState(h_last)
 
 
@@ -85,6 +85,4 @@ def gated_scan_chunk(pa: torch.Tensor, px: torch.Tensor, pc1: torch.Tensor, pc2:
         except _lib.Unsupported:
             pass
     a, x, c, b = _gates(pa, px, pc1, pc2, pd, gate_dtype)
-    if state is not None:
-        state = ScanState(state.h.contiguous())
     return scan_chunk(x, a, b, c, state, out_dtype=out_dtype)

@@ -12,6 +12,7 @@ import torch
 from quick_ssm_b200 import _lib, fp8
 from quick_ssm_b200.layers import SSM, SSMFp8, SSMFused, SSMStack, SSMStackFp8
 from quick_ssm_b200.norm import _room_like, add_rms_norm, add_rms_norm_fp8
+from quick_ssm_b200.streaming import ScanState, scan_chunk
 
 from test_fp8 import BF16, F16, F32, U, check_product, gpu, half_step, ids, operands, plain_norm
 from test_fp8_layers import blocks, plain_block, rel
@@ -155,6 +156,20 @@ def test_stack_takes_the_arguments_that_its_blocks_take():
         got = stack(x, **kw)
         # fp32 sums in another order, as above
         assert (got - seq).abs().max() <= 4e-5 * seq.abs().max() and (got - want).abs().max() <= 4e-5 * want.abs().max()
+
+
+@gpu
+@pytest.mark.parametrize("L", [1, 40])
+def test_scan_continues_from_a_state_in_any_layout(L):
+    a, x, b, c = (torch.rand(5, L, 24, device="cuda") for _ in range(4))
+    h = torch.randn(5, 24, device="cuda")
+    y, end = scan_chunk(x, a, b, c, ScanState(h))
+    wide = torch.randn(5, 48, device="cuda")
+    wide[:, ::2] = h
+    for other in (h.t().contiguous().t(), wide[:, ::2], h[:1].expand(5, 24)):
+        want, want_end = (y, end) if torch.equal(other, h) else scan_chunk(x, a, b, c, ScanState(other.clone()))
+        got, got_end = scan_chunk(x, a, b, c, ScanState(other))
+        assert torch.equal(got, want) and torch.equal(got_end.h, want_end.h)
 
 
 # ------------------------------------------------------------------------------------------------
