@@ -336,3 +336,89 @@ def test_products_joined_over_a_cluster_with_columns_that_end_inside_a_warp(shap
     check_product(ys[0], x, w, bias, str(shape))
     assert all(torch.equal(y, ys[0]) for y in ys)
     _lib.check_device_status(synchronize=True)
+
+
+# ------------------------------------------------------------------------------------------------
+# calls of other kinds
+# ------------------------------------------------------------------------------------------------
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in a source, an output and a gradient: rows at both ends and around 2^31 against the formulas,
+    quantised ones against calls on those rows alone."""
+    rows, H = 2_150_000, 1024
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(rows, H, dtype=BF16, device="cuda").normal_(generator=g)
+    w = torch.rand(H, device="cuda", generator=g) + 0.5
+    at = [0, 1, rows // 2, 2 ** 21 - 1, 2 ** 21, 2 ** 21 + 1, rows - 2, rows - 1]
+    few = x[at].contiguous()
+    y, h = add_rms_norm(x, x, w)
+    # few rows take more warps each, whose sums are joined in another order: the bound of the norm's tests
+    ref, want_h, r = plain_norm(few.cpu(), few.cpu(), w.cpu(), 1e-5)
+    assert torch.equal(h[at].cpu(), want_h)
+    assert ((y[at].double().cpu() - ref).abs() <= (half_step(BF16) + (H / 256 + 64) * U) * (1 + 2 ** -8) * ref.abs()).all()
+    rstd = r.float().reshape(-1).cuda()
+    full = torch.ones(rows, device="cuda")
+    full[at] = rstd
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    _lib.add_rmsnorm_bwd(h, w, x, None, full, dx, None, dw)
+    hd, gw = want_h.double(), few.double().cpu() * w.double().cpu()
+    rd = rstd.double().cpu()[:, None]
+    d = rd * gw - hd * rd ** 3 * (hd * gw).mean(-1, keepdim=True)
+    mag = rd * gw.abs() + hd.abs() * rd ** 3 * (hd * gw).abs().mean(-1, keepdim=True)
+    c = (H / 256 + 64 + 3 * (H / 512 + 32)) * U
+    assert ((dx[at].double().cpu() - d).abs() <= half_step(BF16) * (1 + 2 ** -8) * d.abs() + c * mag).all()
+    del y, h, dx, full
+    q, small = fp8.quantize_rows(x), fp8.quantize_rows(few)
+    assert torch.equal(q.values[at].view(torch.uint8), small.values.view(torch.uint8)) and torch.equal(q.scales[at], small.scales)
+    del q
+    wide_w = fp8.quantize_weight(x)
+    band = fp8.quantize_weight(x[128 * 16700:128 * 16700 + 256].clone())
+    assert torch.equal(wide_w.values[128 * 16700:128 * 16700 + 256].view(torch.uint8), band.values.view(torch.uint8))
+    assert torch.equal(wide_w.scales[16700:16702], band.scales)
+    del wide_w, x
+    M, N, K = 110_000, 20_000, 64
+    a, b, _ = operands(M, N, K)
+    out = fp8.matmul_fp8(a, b)
+    tail = [0, M - 300, M - 1]
+    part = fp8.Fp8Rows(a.values[tail], a.scales[tail])
+    check_product(out[tail], part, b, None)
+    _lib.check_device_status(synchronize=True)
+
+
+@gpu
+def test_inference_mode_and_empty_batches():
+    stack = SSMStack(2, 64, 2.0, compute_dtype=BF16).cuda()
+    x = torch.randn(2, 7, 64, device="cuda")
+    want = stack(x)
+    served = SSMStackFp8(stack)
+    y, states = served(x)
+    with torch.inference_mode():
+        assert torch.equal(stack(x), want)
+        y2, states2 = served(x)
+        assert torch.equal(y2, y) and all(torch.equal(a.h, b.h) for a, b in zip(states, states2))
+        served(x[:, :1], states2)
+    for model in (stack, lambda t: served(t)[0]):
+        assert model(x[:0]).shape == (0, 7, 64) and model(x[:, :0]).shape == (2, 0, 64)
+    _, none = served(x[:0])
+    assert all(s.h.shape == (0, 128) for s in none)
+
+
+@gpu
+def test_calls_from_several_host_threads():
+    """Streams and threads of their own, more operands than the maps that a thread keeps."""
+    import concurrent.futures
+    torch.manual_seed(3)
+    stack = SSMStackFp8(blocks(2, 96, 1.5))
+    inputs = [torch.randn(2, 1 + 3 * i, 96, device="cuda") for i in range(24)]
+    want = [stack(x)[0] for x in inputs]
+    torch.cuda.synchronize()
+
+    def work(order):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [(i, stack(inputs[i])[0]) for i in order]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(y, want[i]) for i, y in got)
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, [range(24), range(23, -1, -1), range(0, 24, 2), range(1, 24, 2)]))
+    _lib.check_device_status(synchronize=True)
