@@ -72,6 +72,9 @@ __device__ __forceinline__ void mbar_arrive_if(bool yes, uint32_t bar) {
                  "r"((uint32_t)yes)
                  : "memory");
 }
+// On a barrier of either CTA (`bar` is a cluster address), for consumers of tensor memory: what it orders are loads that
+// tcgen05.wait has completed.  A release at cluster scope would wait for every other access of the warp as well, 1.2 us per
+// block of k.
 __device__ __forceinline__ void mbar_arrive_cluster_if(bool yes, uint32_t bar) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar),
                  "r"((uint32_t)yes)
@@ -202,12 +205,6 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
     return remote;
-}
-// Arrival on a barrier of either CTA (`bar` is a cluster address), for consumers of tensor memory: what it orders are
-// loads that tcgen05.wait has completed.  A release at cluster scope would wait for every other access of the warp as
-// well, 1.2 us per block of k.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
     float v;
