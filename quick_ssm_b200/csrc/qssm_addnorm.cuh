@@ -7,9 +7,9 @@
 // see the h that the norm saw.  Sums, r and the arithmetic in between are fp32.
 //
 // All of it is bound by memory: forward 2 reads and 2 writes per element, backward 3 reads and one write (two if x
-// and the residual differ in type).  A row is owned by one warp or by the eight warps of a CTA and stays in
-// registers between its sum of squares and its output, so nothing is read twice; rows of more elements than the
-// registers hold are read again from the h that was just written (L1/L2).
+// and the residual differ in type).  A row is owned by 1, 2, 4 or 8 warps of a CTA and stays in registers between its
+// sum of squares and its output, so nothing is read twice; rows of more elements than eight warps' registers hold are
+// read again from the h that was just written (L1/L2).
 //
 // Columns are dealt to lanes in units: with V = 8 elements per access (16-bit data) a unit is 256 columns, lane l
 // owning columns 8l..8l+7; with V <= 4 it is 128 columns in 4/V accesses of V adjacent elements per lane.  Either way
@@ -17,11 +17,11 @@
 // reduction.  V = 4 serves what has fp32 in it and short rows of 16 bits, V = 2 and 1 rows whose pitch or length allow
 // no more.
 //
-// A row is held by 1, 2, 4 or 8 warps, 16 elements a lane (the backward keeps three values of each, packed as they came,
-// and the dw sums), which leaves room for 16 to 32 warps on an SM; a warp takes several rows of one unit at a time.
-// Measured on a B200 against the copy rate (6.54 TB/s), bf16 65536x1024: forward 88 us of 82, to e4m3 82 of 72,
-// backward 105 of 82 (32 elements a lane as floats, eight warps on an SM: 187; the next row not fetched ahead: 113, and
-// to e4m3 104); fp32 166 of 164, 132 of 133, 167 of 164.
+// A lane holds 16 elements of a row (the backward keeps three values of each, packed as they came, and the dw sums), which
+// leaves room for 16 to 32 warps on an SM; a warp takes several rows of one unit at a time.
+// Measured on a B200 against the copy rate (6.54 TB/s), bf16 65536x1024: forward 89 us of 82, to e4m3 84 of 72,
+// backward 104 of 82 (32 elements a lane as floats, eight warps on an SM: 187; the next row not fetched ahead: 113, and
+// to e4m3 104); fp32 165 of 164, 133 of 133, 167 of 164; bf16 on an fp32 stream 125 of 123, 115 of 113, 172 of 164.
 #pragma once
 #include "qssm_elem.cuh"
 

@@ -82,8 +82,10 @@ struct MatmulPlan {
 
 // Which kernel, and over how many CTAs a tile's k is cut: the shortest of these estimates in microseconds, fitted on a
 // B200 with CUDA graphs of 20 calls (N x K 1024x4096, 20480x1024, 4096x4096, 300x16384, 16384x512, 2500x1100, M 1 to
-// 4096).  Both sides there, many-rows / few-rows kernel: 64x1024x4096 19.5 / 8.3, 128x20480x1024 13.9 / 17.8,
-// 64x20480x1024 13.5 / 10.5, 1024x4096x4096 21.8 / 41.5, 512x300x16384 66.3 / 15.5.
+// 4096) to an earlier form of the kernels.  Measured since, many-rows / few-rows kernel: 1x20480x1024 14.4 / 7.1,
+// 64x1024x4096 18.9 / 7.6, 64x20480x1024 14.6 / 10.6, 128x20480x1024 15.2 / 17.9, 1024x4096x4096 20.9 / 41.2, 512x300x16384
+// 58.2 / 15.3, 1537x2500x1100 11.2 / 19.8: the faster one is chosen each time.  The estimates are 6 to 22 % short of the
+// many-rows kernel's times (16384x20480x1024 329 of 373) and within 15 % of the few-rows kernel's.
 //   many rows: 0.47 per block of k and round of tiles over the pairs of SMs, 0.9 to end a round (0.7, 1.9, 5.6 more where
 //              the rows of y take words of 8, 4, 2 bytes only), 3 to begin;
 //   few rows:  0.35 to 0.65 per block of k, 1 per round, 4 to begin, 0.6 to join k.  Clusters of 2, 4 and 8 CTAs are

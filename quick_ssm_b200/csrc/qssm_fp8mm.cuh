@@ -55,11 +55,12 @@ __device__ __forceinline__ float2 as_pair(uint32_t a, uint32_t b) { return make_
 // tile's bias ahead.  Results leave through shared memory and bulk stores of 32 rows x 128 bytes per warp, so that the
 // sums' registers are free for the next tile at once.
 //
-// 16384x20480x1024 374 us, 1.84 PFLOP/s (429 us under the power limit, 1.54 GHz); 16384x1024x4096 71 us;
+// 16384x20480x1024 372 us, 1.85 PFLOP/s (429 us under the power limit, 1.54 GHz); 16384x1024x4096 70 us;
 // 16384x8192x8192 1.1 ms.  The sums' loop has few branches for the same reason: the next block's scales are read in the
-// shadow of the second pair of reads, and the barriers are handed on by predicated arrivals.  One product of 256 columns
-// and one issuing warp per block: 391 us (450); one issuing warp for all buffers: 438 us; sixteen warps of 64 columns:
-// 426 us; tiles of 128 x 256 by single CTAs whose sums fetch their own scales: 835 us.
+// shadow of the second pair of reads, and the barriers are handed on by predicated arrivals (the warps agreeing on each
+// wait's outcome in that loop: 379 us, 72 us).  One product of 256 columns and one issuing warp per block: 391 us (450); one
+// issuing warp for all buffers: 438 us; sixteen warps of 64 columns: 426 us.  Tiles of 128 x 256 by single CTAs took 835 us
+// in an earlier form whose sums fetched their own scales; they were not measured in this one.
 // ---------------------------------------------------------------------------------------------
 constexpr int MMR_M = 256, MMR_N = 256, MMR_STAGES = 4;        // a pair's tile
 constexpr int MMR_A = 128 * MM_TILE_K, MMR_STAGE = 2 * MMR_A;  // per CTA
@@ -334,8 +335,9 @@ template <typename T> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds_
 // Few rows: the weight is the first operand.  Tiles of 128 columns of y x T rows (T = 16 to 128), lane = column, so
 // the weight's rows fill the tensor cores' 128 lanes however few rows there are, and k is cut over the S CTAs of a
 // cluster, whose sums are added in rank order through distributed shared memory (each CTA adds every S-th row).
-// Bound by latencies: a CTA sees few blocks of k, each a copy, a product and a read back.  1x20480x1024 7.2 us,
-// 64x1024x4096 7.4 us (the many-rows kernel 14.7 and 19.5).
+// Bound by latencies: a CTA sees few blocks of k, each a copy, a product and a read back, behind some 4 us of launch and
+// set-up.  1x20480x1024 7.1 us (160 CTAs of eight blocks, k not cut), 64x1024x4096 7.6 us (64 CTAs of four blocks and the
+// join); the many-rows kernel 14.4 and 18.9.
 // ---------------------------------------------------------------------------------------------
 template <int T> struct Few {
     static constexpr int A = 128 * MM_TILE_K, STAGE = A + T * MM_TILE_K;

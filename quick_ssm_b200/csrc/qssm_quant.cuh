@@ -182,7 +182,8 @@ template <typename T, int V> __global__ void __launch_bounds__(256) quant_blocks
 }
 
 // Blocks of 16-bit weights: eight elements a lane and access, 16 lanes to a row, kept as they came.  ANY: rows start
-// anywhere.  65536x1024 bf16 48 us, 65536x1023 62; four (one) at a time 58 (205).
+// anywhere.  65536x1024 bf16 46 us, 65536x1023 58; four (one) at a time 58 (205).  Bound by latency: a CTA has one block,
+// and nothing is on its way while that is reduced and written.
 template <typename T, bool ANY> __global__ void __launch_bounds__(256) quant_blocks16_kernel(const QuantParams p) {
     constexpr int PER = 16, TIMES = FP8_BLOCK / PER;  // rows at a time
     using U = QuantUnit<T, 8>;

@@ -147,7 +147,8 @@ class SSMFp8(nn.Module):
     """An ``SSM`` block for serving, its projections in 8 bits (``fp8.matmul_fp8``): made from a trained block with
     ``SSMFp8(block)``.  One pass is five kernels for a prompt and for a single token alike: residual sum, norm and
     quantisation; the five input projections as one product; the scan with its gates and a carried state; quantisation;
-    the output projection.  No gradient.
+    the output projection.  A state size whose bytes in ``act_dtype`` are no multiple of 16 cannot be sliced for the fused
+    scan: its gates are torch's element-wise kernels then.  No gradient.
 
     ``forward(x, residual, state)`` takes the previous block's output and the residual stream apart (``residual=None``:
     x is the stream itself) and returns ``(out, residual, state)``; the stream behind this block is ``out + residual``.
