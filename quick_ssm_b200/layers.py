@@ -91,11 +91,11 @@ class SSMFused(SSM):
         return self._branch(self._normed(x) if self.use_norm else x, scan_out_dtype) + skip
 
     def _normed(self, x: torch.Tensor) -> torch.Tensor:
-        """The normalisation kernels on the layer's own weight.  They keep x's type; the plain norm's product promotes x to
-        the weight's, which the projections ask for unless autocast chooses their type."""
+        """The normalisation kernels on the layer's own weight.  They keep x's type, where the plain norm's product promotes x
+        to the weight's: so does this one where the projections are in another type than x and autocast does not see to it."""
         from .norm import rms_norm
         w = self.pre_norm.weight
-        if x.dtype != w.dtype and not torch.is_autocast_enabled("cuda"):
+        if x.dtype != self.out_proj.weight.dtype and not torch.is_autocast_enabled("cuda"):
             x = x.to(torch.promote_types(x.dtype, w.dtype))
         return rms_norm(x, w, self.pre_norm.eps)
 

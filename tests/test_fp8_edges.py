@@ -145,6 +145,18 @@ def test_stack_takes_the_types_that_its_blocks_take(weights, xd):
 
 
 @gpu
+def test_norm_weights_in_float32_beside_16_bit_projections():
+    """What the fused blocks take and the plain ones do not: the norm on x as it is."""
+    fused, stack = SSMFused(64, dtype=BF16, compute_dtype=BF16).cuda(), SSMStack(2, 64, dtype=BF16, compute_dtype=BF16).cuda()
+    x = torch.randn(2, 9, 64, device="cuda").to(BF16)
+    same = stack(x), fused(x)
+    for layer in (fused, *stack.layers):
+        layer.pre_norm.float()  # ones either way
+    for got, want in zip((stack(x), fused(x)), same):
+        assert got.dtype == BF16 and torch.equal(got, want)
+
+
+@gpu
 def test_stack_takes_the_arguments_that_its_blocks_take():
     stack = SSMStack(2, 32, compute_dtype=F32).cuda()
     x = torch.randn(2, 40, 32, device="cuda")
