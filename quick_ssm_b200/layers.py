@@ -214,6 +214,8 @@ class SSMFp8(nn.Module):
         from .fp8 import matmul_fp8, quantize_rows
         from .norm import add_rms_norm_fp8
         from .streaming import gated_scan_chunk
+        if residual is not None and residual.dtype not in (x.dtype, torch.float32):  # as their sum would be promoted
+            residual = residual.float()
         u, h = add_rms_norm_fp8(x, residual, self.norm_weight, self.eps)
         p = matmul_fp8(u, self._weight("in"), self.in_bias, out_dtype=self.act_dtype)
         y, state = gated_scan_chunk(*p.split(self.state_size_dim, dim=-1), state, gate_dtype=self.gate_dtype)
@@ -242,10 +244,7 @@ class SSMStackFp8(nn.Module):
             raise ValueError("x must be [B, L, hidden]")
         y, h, after = x, None, []
         for layer, state in zip(self.layers, states):
-            # a residual stream in the branch's own type, or in fp32
             y, h, state = layer(y, h, state)
-            if h.dtype not in (y.dtype, torch.float32):
-                h = h.float()
             after.append(state)
         return (h + y).to(x.dtype), after
 

@@ -91,6 +91,20 @@ def test_serving_a_block_of_float16_gates_keeps_the_range_of_its_weights(what):
 
 
 @gpu
+@pytest.mark.parametrize("xd", [F32, BF16, F16], ids=ids)
+@pytest.mark.parametrize("compute", [BF16, F16], ids=ids)
+def test_serving_blocks_chained_by_hand(compute, xd):
+    """Block after block with the residual stream apart, whatever its type: the stack's result."""
+    made = blocks(3, 64, 2.0, compute=compute)
+    x = torch.randn(2, 9, 64, device="cuda").to(xd)
+    want, _ = SSMStackFp8(made)(x)
+    y, h = x, None
+    for block in made:
+        y, h, _ = SSMFp8(block)(y, h)
+    assert want.dtype == xd and torch.equal((h + y).to(xd), want)
+
+
+@gpu
 def test_serving_types_follow_the_block():
     for weights, compute, gate, want in ((F32, F16, None, (F16, F32)), (F32, BF16, None, (BF16, BF16)), (F32, F32, None, (BF16, BF16)),
                                          (F16, F16, None, (F16, F16)), (BF16, F16, None, (F16, F32)), (F32, F16, BF16, (BF16, BF16)),
